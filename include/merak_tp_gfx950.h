@@ -454,6 +454,147 @@ int mtp_attn_decode_append(const void* qkv, const void* cos_table, const void* s
                            float scale, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Serving over a paged key/value cache.  Keys and values live in pages of
+ * page_size tokens, [n_pages, n_kv_heads, page_size, head_dim], that requests
+ * take from a free list as they grow; row r of a block table names the pages
+ * of request r in order, and a token's slot is page * page_size + its place in
+ * the page.  A step: mtp_paged_plan (lengths -> pages, slots, positions),
+ * mtp_qk_norm_rope_append (QKV rows -> rotated queries, keys and values in
+ * their slots), mtp_attn_paged (queries against the pages), and where tokens
+ * were drafted mtp_verify_draft.  The reference has no key/value cache (its
+ * loop re-runs the sequence, text_generation_inference.py:199-203).
+ * Lengths, positions, slots and token offsets are int64, page ids and page
+ * counts int32.  Sizes that live on the device are checked there: a position,
+ * slot or page id out of range is never used as an address.
+ * ------------------------------------------------------------------------ */
+/* For each of `requests` (at most 4096) requests with lens[r] cached tokens,
+ * new_lens[r] arriving ones and held[r] pages in row r of block_tables
+ * [requests, max_pages]: takes the pages it lacks from the top of the free
+ * list (free_pages[free_capacity], free_count[0] of them free) in request
+ * order, writes them behind the held ones in the table, and gives
+ *   cu [requests + 1]   exclusive prefix sums of new_lens (where the tokens of
+ *                       a request start among all new tokens)
+ *   slots, positions [tokens]  cache slot and position of each new token;
+ *                       -1 behind the last token and for refused requests
+ *   kv_lens [requests]  lens + new_lens, 0 for refused requests
+ *   granted [requests]  1, or 0 = refused: a request that needs pages when the
+ *                       running sum of pages needed passes the free ones, whose
+ *                       length would pass max_pages * page_size, whose tokens
+ *                       end behind `tokens`, or whose lens or held is out of
+ *                       range; its pages and counts stay as they were
+ *   held_out, free_count_out  the new counts, in buffers of their own (the free
+ *                       list itself is unchanged: its top moved).
+ * A negative new_lens counts as 0.  page_size is a power of two,
+ * max_pages * page_size < 2^31.  Equal inputs give equal outputs, however often
+ * the call is repeated. */
+int mtp_paged_plan(const int64_t* lens, const int64_t* new_lens, const int32_t* held,
+                   int32_t* block_tables, const int32_t* free_pages, const int32_t* free_count,
+                   int64_t* slots, int64_t* positions, int64_t* cu, int64_t* kv_lens,
+                   uint8_t* granted, int32_t* held_out, int32_t* free_count_out,
+                   int64_t requests, int64_t max_pages, int64_t page_size,
+                   int64_t free_capacity, int64_t tokens, void* stream);
+
+/* The pages of every request with finished[r] != 0 go back on the free list,
+ * in request and table order; held[r] becomes 0 and free_count grows.  A
+ * request whose pages the list has no room for keeps them (a page that never
+ * came from the list). */
+int mtp_paged_release(const uint8_t* finished, int32_t* held, const int32_t* block_tables,
+                      int32_t* free_pages, int32_t* free_count,
+                      int64_t requests, int64_t max_pages, int64_t free_capacity, void* stream);
+
+/* RMSNorm of each query and key head and rotary embedding, in one pass.
+ * qkv [T, (n_q_heads + 2 n_kv_heads) * head_dim]: query heads, key heads, value
+ * heads.  For a head x at position p, with z = weight * x / sqrt(mean(x^2) +
+ * eps) (z = x where the weight of its kind is NULL): y = z * cos[p] +
+ * rotate_half(z) * sin[p] (HF apply_rotary_pos_emb), in fp32, rounded once.
+ * q_out [T, n_q_heads, head_dim], k_out [T, n_kv_heads, head_dim].  Tables
+ * [max_positions, head_dim], fp32 or the tensors' type (table_dtype); weights
+ * [head_dim] of the tensors' type.  A row whose position is outside the tables
+ * gives zeros.  head_dim 64 or 128; f32, bf16 or f16; T <= 2^21. */
+int mtp_qk_norm_rope(const void* qkv, const void* cos_table, const void* sin_table, int table_dtype,
+                     const int64_t* positions, const void* q_weight, const void* k_weight,
+                     void* q_out, void* k_out,
+                     int64_t T, int n_q_heads, int n_kv_heads, int head_dim, int64_t max_positions,
+                     float eps, int dtype, void* stream);
+
+/* Its backward: dqkv [T, (n_q_heads + 2 n_kv_heads) * head_dim] whole, dv
+ * copied into the values' place; dq, dk or dv NULL: zeros.  dq_weight and
+ * dk_weight [head_dim] (each may be NULL) are summed over all rows in a fixed
+ * order (the same bits on every run) through the workspace, which needs
+ * mtp_qk_norm_rope_bwd_workspace_bytes(...) bytes when either is wanted; its
+ * contents on entry do not matter.  A row whose position is outside the tables
+ * adds nothing and gets zeros for its queries and keys. */
+int64_t mtp_qk_norm_rope_bwd_workspace_bytes(int64_t T, int n_q_heads, int n_kv_heads, int head_dim);
+int mtp_qk_norm_rope_bwd(const void* dq, const void* dk, const void* dv, const void* qkv,
+                         const void* cos_table, const void* sin_table, int table_dtype,
+                         const int64_t* positions, const void* q_weight, const void* k_weight,
+                         void* dqkv, void* dq_weight, void* dk_weight,
+                         void* workspace, int64_t workspace_bytes,
+                         int64_t T, int n_q_heads, int n_kv_heads, int head_dim, int64_t max_positions,
+                         float eps, int dtype, void* stream);
+
+/* The serving form: queries to q_out, keys (normed and rotated) and values
+ * (copied) to slots[t] of k_cache and v_cache [n_pages, n_kv_heads, page_size,
+ * head_dim].  A row whose slot is outside the cache, or whose position is
+ * outside the tables, appends nothing.  Two rows with one slot: one of them
+ * stays, which is not said.  bf16 or f16; page_size a power of two. */
+int mtp_qk_norm_rope_append(const void* qkv, const void* cos_table, const void* sin_table, int table_dtype,
+                            const int64_t* positions, const int64_t* slots,
+                            const void* q_weight, const void* k_weight,
+                            void* q_out, void* k_cache, void* v_cache,
+                            int64_t T, int n_q_heads, int n_kv_heads, int head_dim, int64_t max_positions,
+                            int64_t n_pages, int64_t page_size, float eps, int dtype, void* stream);
+
+/* Causal attention of the new tokens of each request over its pages.  Request
+ * r owns rows cu[r] .. cu[r+1]-1 of q and out [T, n_q_heads, head_dim]; its
+ * last new token is token kv_lens[r] - 1 of its cache, so row i of its n rows
+ * sees the tokens up to kv_lens[r] - n + i:
+ *   out[i,h,:] = softmax_t(scale * q[i,h,:] . K[t,h/g,:]) V[t,h/g,:]
+ * with g = n_q_heads / n_kv_heads <= 32; one row that sees nothing gives
+ * zeros.  Any mix of single tokens, drafts and prompts.  Scores, softmax and
+ * sums are fp32; probabilities are rounded to the tensor type for the product
+ * with V.  Rows of no request are left as they were.  cu, kv_lens: int64 on the
+ * device; kv_lens is clamped to the table row, cu to T.  Tokens whose page id is
+ * outside the cache read as zeros.  What lies in a page behind a request's
+ * length is not read into the result, whatever it holds; keys and values below
+ * it are expected to be finite.
+ * max_new bounds the new tokens of a request and len_bound kv_lens, both known
+ * on the host; they choose how work is laid out, and a request that passes
+ * max_new is still computed.  workspace:
+ * mtp_attn_paged_workspace_bytes() bytes for any shape, 16-byte aligned; ITS
+ * FIRST 4096 BYTES MUST BE ZERO before the first launch that uses it and are
+ * zero again after each.  Launches that share a workspace must not overlap.
+ * head_dim 64 or 128; bf16 or f16; page_size a power of two, at least 16. */
+int64_t mtp_attn_paged_workspace_bytes(void);
+int mtp_attn_paged(const void* q, const void* k_cache, const void* v_cache,
+                   const int32_t* block_tables, const int64_t* cu, const int64_t* kv_lens, void* out,
+                   void* workspace, int64_t workspace_bytes,
+                   int64_t T, int64_t requests, int n_q_heads, int n_kv_heads, int head_dim,
+                   int64_t n_pages, int64_t page_size, int64_t max_pages,
+                   int64_t max_new, int64_t len_bound, float scale, int dtype, void* stream);
+
+/* Verification of drafted tokens (K <= 64 per request) against the target's
+ * probabilities: draft i of request r is accepted while
+ *   uniforms[r,i] * draft_probs[r,i,x] < target_probs[r,i,x],  x its token;
+ * after n accepted ones the next token is the first index whose cumulative
+ * weight exceeds uniforms[r,K] times the sum of the weights, in index order,
+ * with the weights max(target_probs[r,n] - draft_probs[r,n], 0) after a
+ * rejection (target_probs[r,n] where those are all zero) and target_probs[r,n]
+ * when nothing was rejected.  tokens [R, K+1]: accepted drafts, the drawn
+ * token, then -1; accepted [R] = n.  draft_lens (NULL: K each) limits the
+ * drafts of a request.  draft_probs NULL: the drafts were certain (probability
+ * 1 on x).  target_probs [R, K+1, V], draft_probs [R, K, V] of f32, bf16 or
+ * f16, not necessarily normalised; weights that are not positive and finite
+ * count as zero, a row without any weight draws -1; a draft outside [0, V) is
+ * rejected.  uniforms f32 [R, K+1] in [0, 1).  Products and sums are fp64.
+ * workspace: mtp_verify_draft_workspace_bytes(R, V) bytes, 8-byte aligned. */
+int64_t mtp_verify_draft_workspace_bytes(int64_t R, int64_t V);
+int mtp_verify_draft(const int64_t* draft_tokens, const int64_t* draft_lens,
+                     const void* target_probs, const void* draft_probs, const float* uniforms,
+                     int64_t* tokens, int64_t* accepted, void* workspace, int64_t workspace_bytes,
+                     int64_t R, int K, int64_t V, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------
  * Measurement helpers (used by bench.py to state what this GPU can do).
  * ------------------------------------------------------------------------ */
 /* The library reads its MTP_* tuning variables (tile and slice choices that

@@ -67,6 +67,20 @@ SIGNATURES = {
     "mtp_attn_decode": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _int, _int, _i64, _i64, C.c_float, _int, _vp]),
     "mtp_attn_decode_append": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _int, _int, _i64, _i64, _i64,
                                       C.c_float, _int, _vp]),
+    "mtp_paged_plan": (_int, [_vp] * 13 + [_i64] * 5 + [_vp]),
+    "mtp_paged_release": (_int, [_vp] * 5 + [_i64] * 3 + [_vp]),
+    "mtp_qk_norm_rope": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _i64, _int, _int, _int, _i64, C.c_float, _int,
+                                _vp]),
+    "mtp_qk_norm_rope_bwd_workspace_bytes": (_i64, [_i64, _int, _int, _int]),
+    "mtp_qk_norm_rope_bwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int,
+                                    _int, _int, _i64, C.c_float, _int, _vp]),
+    "mtp_qk_norm_rope_append": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _int, _int, _int, _i64,
+                                       _i64, _i64, C.c_float, _int, _vp]),
+    "mtp_attn_paged_workspace_bytes": (_i64, []),
+    "mtp_attn_paged": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _int, _i64, _i64, _i64,
+                              _i64, _i64, C.c_float, _int, _vp]),
+    "mtp_verify_draft_workspace_bytes": (_i64, [_i64, _i64]),
+    "mtp_verify_draft": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _i64, _int, _vp]),
     "mtp_reload_tuning": (None, []),
     "mtp_stream_copy": (_int, [_vp, _vp, _i64, _vp]),
     "mtp_mfma_peak": (_int, [_vp, _i64, _i64, _int, _vp]),

@@ -39,6 +39,7 @@ SOURCES = [
     "gemm_bf16_wgrad.hip",
     "gemm_generic.hip", "gemm_f32.hip", "decode_attn.hip",
     "linear.hip",
+    "paged_plan.hip", "qk_norm_rope.hip", "attn_paged.hip", "verify_draft.hip",
 ]
 
 # -packed-fp32-ops off: packed fp32 VALU forms are not to be generated for this target pool.

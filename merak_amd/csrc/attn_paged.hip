@@ -1,0 +1,795 @@
+// Causal grouped-query attention of the new tokens of many requests over a paged key/value cache, for gfx950: one
+// operator for single tokens, drafted tokens and prompts, in any mix.
+//
+//   out[i,h,:] = sum_t p_t V[t,:] / sum_t p_t,   p_t = exp(scale q[i,h,:] . K[t,:] - max),   t <= kv_len - n + i
+//
+// in one pass over the keys and values with the running maximum m and sum l of a softmax, in fp32.
+//
+// Rows.  The g = n_q / n_kv query heads of a key head read the same keys: the rows of a tile are (token, head of the
+// group) pairs, token major, so a tile of one request and one key head has n g rows whatever n is, and reads each key
+// once for all of them.
+//
+// Products.  S^T = K Q^T and O^T = V^T P^T with v_mfma_f32_32x32x16: a lane then owns one row (column lane % 32 of the
+// result), the maximum and the sum of a row are in-lane plus one exchange with lane ^ 32, and the 16 scores of a lane
+// already sit where the second product takes its right operand, in the k order  4h + {0..3}, 8 + 4h + {0..3}  of each
+// 16 tokens (h = lane / 32) - the transposed reads of V follow the same order, so P never moves.
+//
+// Keys and values go global -> LDS by DMA in blocks of 16 tokens (a page holds at least 16): the block's page id is a
+// scalar load, its 64-bit address the base of a buffer resource whose range ends at the request's last token, so
+// tokens behind it read as zeros whatever lies there, and an unknown page reads as zeros too.  16-byte chunk c of token
+// t sits at chunk position c ^ swz(t) of its row: the fragment reads of K (8 rows, one chunk) and the transposed reads
+// of V (4 rows, two neighbouring chunks) then fall into different banks.
+//
+// Work.  The key/value range of every (request, key head, tile) is counted in units (32 or 64 tokens) plus a constant
+// for the tile's start, and the whole sequence of units is dealt to the workgroups in equal runs: lengths may differ by
+// any factor, a long context is split over as many workgroups as its share, short ones share a workgroup, and nothing
+// depends on what the host knows of the lengths.  Every workgroup finds its run by itself (a prefix sum over the
+// requests).  A tile that is cut leaves partial results (O, m, l) in the workspace; the workgroup that delivers last
+// merges them in order, so the result does not depend on which one that is.
+//
+// Two kernels, chosen by the most rows a tile can have:
+//   narrow  up to 32 RB rows (RB = 1, 2), bound by HBM: the waves of a workgroup take turns with the units of its run,
+//           each with a ring of LDS slots of its own and no barrier in the loop, and are merged at the end;
+//   wide    128 rows, 32 per wave, bound by the matrix cores: the waves share each unit's keys and values.
+#include "gemm_bf16_kernel.h"
+
+namespace {
+
+constexpr int AP_PAGE_MIN = 16;      // tokens per DMA block
+constexpr int AP_START = 2;          // a tile's start (queries, merge, output) in units
+constexpr int AP_MAX_WGS = 1024;     // arrival counters: 4 bytes each at the head of the workspace
+constexpr int64_t AP_COUNTER_BYTES = 4096;
+
+struct PagedArgs {
+  const uint16_t* q;         // [T, n_q, D]
+  const uint16_t* k;         // [n_pages, n_kv, page_size, D]
+  const uint16_t* v;
+  const int32_t* table;      // [requests, max_pages]
+  const int64_t* cu;         // [requests + 1]
+  const int64_t* kv_lens;    // [requests]
+  uint16_t* out;
+  float* part;               // [2 wgs] partial tiles
+  int32_t* arrived;          // [wgs] zero between launches
+  int64_t max_pages;
+  int T, requests, n_q, n_kv, group, page_shift, n_pages, room, wgs, min_units;
+  float scale_log2e;
+};
+
+// uniform, read-only data: scalar loads
+template <typename T> __device__ __forceinline__ T scalar_load(const T* p) {
+  return *(const T __attribute__((address_space(4)))*)(uintptr_t)p;
+}
+
+// a value that is the same in every lane, in scalar registers
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+                   (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+
+__device__ __forceinline__ void ap_store(float* p, float v) {   // served at the level all XCDs share
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float ap_load(const float* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+template <int N> __device__ __forceinline__ void wait_vm_at_most() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// ---- the sequence of units -----------------------------------------------------------------------------
+struct Request {
+  int t0, n, kv;             // first row's token, new tokens, cached tokens with them
+};
+__device__ __forceinline__ int clamp64(int64_t v, int hi) { return v < 0 ? 0 : v > hi ? hi : (int)v; }
+__device__ __forceinline__ Request request_of(const PagedArgs& p, int r) {
+  const int a = clamp64(scalar_load(p.cu + r), p.T), b = clamp64(scalar_load(p.cu + r + 1), p.T);
+  return Request{a, b > a ? b - a : 0, clamp64(scalar_load(p.kv_lens + r), p.room)};
+}
+
+// Walks the tiles of a request: tokens that the tile's last row may see, in units of TK.
+template <int BM, int TK>
+struct Tiles {
+  int e0, n, kv, whole, rest, tok, frac, group;
+  __device__ __forceinline__ Tiles(const Request& q, int g) {
+    e0 = q.kv - q.n;
+    n = q.n;
+    kv = q.kv;
+    group = g;
+    whole = BM / g;
+    rest = BM % g;
+    tok = frac = 0;
+  }
+  __device__ __forceinline__ int next() {     // units of the next tile
+    tok += whole;
+    frac += rest;
+    if (frac >= group) {
+      frac -= group;
+      tok++;
+    }
+    const int upto = tok + (frac > 0 ? 1 : 0);
+    const int end = e0 + (upto < n ? upto : n);
+    return end <= 0 ? 0 : (end + TK - 1) / TK;
+  }
+};
+
+struct Run {                 // a workgroup's run of the sequence, and where it starts
+  int64_t x, hi, total;      // cost positions
+  int wgs;                   // workgroups that have a run
+  int r;
+  int64_t head_cost, off;    // cost of one key head of request r, position inside the request
+};
+
+template <int BM, int TK, int THREADS>
+__device__ __forceinline__ bool find_run(const PagedArgs& p, int w, Run& run) {
+  __shared__ int64_t sums[THREADS / 64];
+  __shared__ int64_t found[3];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int per = (p.requests + THREADS - 1) / THREADS;
+  const int r0 = tid * per < p.requests ? tid * per : p.requests;
+  const int r1 = r0 + per < p.requests ? r0 + per : p.requests;
+  auto cost_of = [&](int r) -> int64_t {      // of one key head
+    const Request q = request_of(p, r);
+    const int tiles = (int)(((int64_t)q.n * p.group + BM - 1) / BM);
+    Tiles<BM, TK> walk(q, p.group);
+    int64_t c = 0;
+    for (int j = 0; j < tiles; j++) c += walk.next() + AP_START;
+    return c;
+  };
+  int64_t own = 0;
+  for (int r = r0; r < r1; r++) own += cost_of(r);
+  int64_t incl = own;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t up = __shfl_up((long long)incl, o, 64);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 63) sums[wave] = incl;
+  __syncthreads();
+  int64_t base = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; i++) {
+    if (i < wave) base += sums[i];
+    total += sums[i];
+  }
+  total = uniform(total * p.n_kv);
+  int64_t at = (base + incl - own) * p.n_kv;
+  const int64_t most = (total + p.min_units - 1) / p.min_units;
+  const int wgs = most < p.wgs ? (int)most : p.wgs;
+  if (w >= wgs) return false;                 // the same for the whole workgroup
+  const int64_t lo = total * w / wgs;
+  if (at <= lo && lo < at + own * p.n_kv) {
+    for (int r = r0; r < r1; r++) {
+      const int64_t c = cost_of(r);
+      if (lo < at + c * p.n_kv) {
+        found[0] = r;
+        found[1] = c;
+        found[2] = lo - at;
+        break;
+      }
+      at += c * p.n_kv;
+    }
+  }
+  __syncthreads();
+  run.x = lo;
+  run.hi = total * (w + 1) / wgs;
+  run.total = total;
+  run.wgs = wgs;
+  run.r = __builtin_amdgcn_readfirstlane((int)found[0]);
+  run.head_cost = uniform(found[1]);
+  run.off = uniform(found[2]);
+  return true;
+}
+// workgroup whose run holds position x: the largest w with floor(total w / wgs) <= x
+__device__ __forceinline__ int wg_of(const Run& run, int64_t x) { return (int)(((x + 1) * run.wgs - 1) / run.total); }
+
+// ---- one wave's share of the products -----------------------------------------------------------------
+// position of a 16-byte chunk in its token's row of the LDS tile
+template <int D> __device__ __forceinline__ int swz(int t) {
+  if (D == 128) return ((t & 7) << 1) | ((t >> 3) & 1);
+  return (((t >> 1) & 3) << 1) | ((t >> 3) & 1);       // two rows share the 256 bytes of the banks
+}
+
+template <int D, bool F16, int RB, int NB>
+struct Wave {
+  using X = X16<F16>;
+  static constexpr int KS = D / 16, DT = D / 32, ROW = D * 2;
+  bf16x8_t qf[RB][KS];
+  f32x16_t o[RB][DT];
+  float m[RB], l[RB];
+  int lim[RB];               // first token the lane's row does not see
+  u32x4_t pf[RB][2 * NB];    // probabilities of the unit, as the second product's operand
+
+  // rows row0 + 32 rb + lane % 32 of the tile, of which `rows` exist
+  __device__ __forceinline__ void start(const PagedArgs& p, const Request& q, int kvh, int row0, int rows) {
+    const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) {
+      int row = row0 + 32 * rb + c;
+      if (row >= rows) row = rows - 1;        // a copy of the last row, never stored
+      const int tok = row / p.group, g = row - tok * p.group;
+      const uint16_t* src = p.q + ((int64_t)(q.t0 + tok) * p.n_q + kvh * p.group + g) * D + 8 * h;
+#pragma unroll
+      for (int s = 0; s < KS; s++) qf[rb][s] = *reinterpret_cast<const bf16x8_t*>(src + 16 * s);
+      lim[rb] = q.kv - q.n + tok + 1;
+      m[rb] = -INFINITY;
+      l[rb] = 0.0f;
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[rb][dt][i] = 0.0f;
+    }
+  }
+
+  // scores of the unit's keys (LDS tile `ks`, first token tok0), running maximum and sum, probabilities
+  __device__ __forceinline__ void scores(const char* ks, int tok0, bool mask, float c) {
+    const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
+    f32x16_t s[RB][NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      const char* base = ks + (32 * b + row) * ROW;
+#pragma unroll
+      for (int rb = 0; rb < RB; rb++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[rb][b][i] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KS; k++) {
+        const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(base + (((2 * k + h) ^ swz<D>(row)) << 4));
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) s[rb][b] = X::mfma32(a, qf[rb][k], s[rb][b]);
+      }
+    }
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) {
+      if (mask) {
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            if (tok0 + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) >= lim[rb]) s[rb][b][i] = -INFINITY;
+      }
+      float mx = s[rb][0][0];
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[rb][b][i]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      // The maximum only has to keep the exponentials in range: it is moved (and O and l rescaled) when a row's has
+      // grown by more than 8 binary orders, not at every step.  A row that has seen nothing yet stays at -inf.
+      if (__any((mx - m[rb]) * c > 8.0f)) {
+        const float mn = fmaxf(m[rb], mx);
+        const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m[rb] - mn) * c);
+        m[rb] = mn;
+        l[rb] *= f;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) o[rb][dt][i] *= f;
+      }
+      const float mc = m[rb] == -INFINITY ? 0.0f : m[rb] * c;
+      float sum = 0.0f;
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          s[rb][b][i] = __builtin_amdgcn_exp2f(fmaf(s[rb][b][i], c, -mc));
+          sum += s[rb][b][i];
+        }
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) pf[rb][2 * b + k][e] = X::pack2(s[rb][b][8 * k + 2 * e], s[rb][b][8 * k + 2 * e + 1]);
+      }
+      l[rb] += sum;
+    }
+  }
+
+  // O^T += V^T P^T from the unit's values (LDS tile `vs`)
+  __device__ __forceinline__ void values(const char* vs) {
+    const int lane = threadIdx.x & 63, i16 = lane & 15, half = (lane >> 4) & 1, h = lane >> 5;
+    const int t = 4 * h + (i16 >> 2);
+#pragma unroll
+    for (int k = 0; k < 2 * NB; k++) {
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++) {
+        const int chunk = 4 * dt + 2 * half + ((i16 & 3) >> 1);
+        const char* a = vs + (16 * k + t) * ROW + ((chunk ^ swz<D>(t)) << 4) + 8 * (i16 & 1);
+        const char* b = vs + (16 * k + t + 8) * ROW + ((chunk ^ swz<D>(t + 8)) << 4) + 8 * (i16 & 1);
+        const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((bf16x4_t __attribute__((address_space(3)))*)(a));
+        const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((bf16x4_t __attribute__((address_space(3)))*)(b));
+        const bf16x8_t vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) o[rb][dt] = X::mfma32(vf, __builtin_bit_cast(bf16x8_t, pf[rb][k]), o[rb][dt]);
+      }
+    }
+  }
+
+  // row block rb as fp32 [32][D + 4] (padded: rows start in different banks) and (m, l) per row
+  __device__ __forceinline__ void to_lds(int rb, float* dst, float* ml) const {
+    const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        *reinterpret_cast<f32x4_t*>(dst + row * (D + 4) + 32 * dt + 8 * i + 4 * h) =
+            f32x4_t{o[rb][dt][4 * i], o[rb][dt][4 * i + 1], o[rb][dt][4 * i + 2], o[rb][dt][4 * i + 3]};
+    const float sum = l[rb] + __shfl_xor(l[rb], 32, 64);
+    if (h == 0) {
+      ml[2 * row] = m[rb];
+      ml[2 * row + 1] = sum;
+    }
+  }
+};
+
+// DMA of one block of 16 tokens (keys or values) into LDS; `voff` from block_offsets
+template <int D> constexpr int block_dmas() { return AP_PAGE_MIN * D * 2 / 1024; }
+template <int D> __device__ __forceinline__ void block_offsets(uint32_t* voff) {
+  const int lane = threadIdx.x & 63;
+  constexpr int CHUNKS = D / 8, ROWS = 64 / CHUNKS;    // chunks per row, rows per DMA instruction
+#pragma unroll
+  for (int j = 0; j < block_dmas<D>(); j++) {
+    const int t = ROWS * j + lane / CHUNKS;
+    voff[j] = (uint32_t)(t * D * 2 + (((lane % CHUNKS) ^ swz<D>(t)) << 4));
+  }
+}
+template <int D>
+__device__ __forceinline__ void dma_block(const uint16_t* cache, int64_t offset, int tokens, uint32_t lds_addr, const uint32_t* voff) {
+  const rsrc_t v = make_rsrc(cache + offset, (int64_t)tokens * (D * 2));
+  const rsrc_t r = {__builtin_amdgcn_readfirstlane(v[0]), __builtin_amdgcn_readfirstlane(v[1]),
+                    __builtin_amdgcn_readfirstlane(v[2]), v[3]};
+#pragma unroll
+  for (int j = 0; j < block_dmas<D>(); j++) dma16(r, lds_addr + j * 1024, voff[j], 0);
+}
+
+// page of the block of 16 tokens at tok, -1 when it is unknown or the request ends before
+__device__ __forceinline__ int page_at(const PagedArgs& p, int r, int kv, int tok) {
+  if (tok >= kv) return -1;
+  const int page = scalar_load(p.table + (int64_t)r * p.max_pages + (tok >> p.page_shift));
+  return page >= 0 && page < p.n_pages ? page : -1;
+}
+// element offset of the block and the tokens of it that exist
+template <int D>
+__device__ __forceinline__ int64_t block_at(const PagedArgs& p, int page, int kvh, int kv, int tok, int& tokens) {
+  const int left = kv - tok;
+  tokens = page < 0 ? 0 : left < AP_PAGE_MIN ? (left < 0 ? 0 : left) : AP_PAGE_MIN;
+  const int64_t in_page = tok & ((1 << p.page_shift) - 1);
+  return ((((int64_t)(page < 0 ? 0 : page) * p.n_kv + kvh) << p.page_shift) + in_page) * D;
+}
+
+// ---- results of a tile --------------------------------------------------------------------------------
+// where partial results of a workgroup go: its first tile (started by an earlier workgroup) and its last (its own)
+__device__ __forceinline__ int64_t slot_of(int w, int first) { return 2 * (int64_t)w + (w == first ? 1 : 0); }
+
+template <int D>
+__device__ __forceinline__ uint16_t* out_row(const PagedArgs& p, const Request& q, int kvh, int row) {
+  const int tok = row / p.group, g = row - tok * p.group;
+  return p.out + ((int64_t)(q.t0 + tok) * p.n_q + kvh * p.group + g) * D;
+}
+
+// what a partial result with maximum m is multiplied with under the common maximum: one that has seen nothing
+// (m = -inf) holds zeros - or NaN, from a NaN in its scores, which has to be seen
+__device__ __forceinline__ float part_scale(float m, float common, float c) {
+  return m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - common) * c);
+}
+
+// After a workgroup has stored its partial tile: the one that delivers last adds all of them up, in order.  Partial
+// results travel by device-coherent accesses, so no cache is written back or invalidated: the workgroup waits until
+// its stores are acknowledged, then counts itself.
+template <int D, bool F16, int BM, int THREADS>
+__device__ __forceinline__ void merge_if_last(const PagedArgs& p, const Request& q, int kvh, int tile, int rows, int first, int last) {
+  using X = X16<F16>;
+  __shared__ int is_last;
+  const int tid = threadIdx.x;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) {
+    const int seen = __hip_atomic_fetch_add(p.arrived + first, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    is_last = seen == last - first;
+    if (is_last) __hip_atomic_store(p.arrived + first, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!is_last) return;
+  constexpr int64_t STRIDE = (int64_t)BM * (D + 2);
+  for (int idx = tid; idx < rows * D; idx += THREADS) {
+    const int row = idx / D, d = idx % D;
+    float mstar = -INFINITY, acc = 0.0f, sum = 0.0f;
+    for (int w0 = first; w0 <= last; w0 += 8) {
+      float mv[8], ov[8], lv[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const int w = w0 + u <= last ? w0 + u : w0;
+        const float* src = p.part + slot_of(w, first) * STRIDE;
+        mv[u] = ap_load(src + BM * D + 2 * row);
+        lv[u] = ap_load(src + BM * D + 2 * row + 1);
+        ov[u] = ap_load(src + row * D + d);
+        if (w0 + u > last) {
+          mv[u] = -INFINITY;
+          lv[u] = ov[u] = 0.0f;
+        }
+      }
+      float mn = mstar;
+#pragma unroll
+      for (int u = 0; u < 8; u++) mn = fmaxf(mn, mv[u]);
+      const float keep = part_scale(mstar, mn, p.scale_log2e);
+      acc *= keep;
+      sum *= keep;
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const float f = part_scale(mv[u], mn, p.scale_log2e);
+        acc += ov[u] * f;
+        sum += lv[u] * f;
+      }
+      mstar = mn;
+    }
+    // a sum that is not positive is a row that sees nothing - or NaN, which has to be seen
+    out_row<D>(p, q, kvh, tile * BM + row)[d] = X::to_bits(sum == 0.0f ? 0.0f : acc / sum);
+  }
+}
+
+// ---- narrow tiles: the waves take turns with the units ------------------------------------------------------
+template <int D, bool F16, int RB, int WAVES, int RING>
+__global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const PagedArgs p) {
+  using X = X16<F16>;
+  constexpr int TK = 32, BM = 32 * RB, THREADS = WAVES * 64;
+  constexpr int ITEM = TK * D * 2, DMAS = ITEM / 1024, AHEAD = RING - 1;
+  static_assert(32 * (D + 4) * 4 <= RING * ITEM && AHEAD * DMAS < 64, "merge area / vmcnt range");
+  __shared__ __attribute__((aligned(1024))) char lds[WAVES * RING * ITEM];
+  __shared__ float ml[WAVES][64];
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int w = blockIdx.x;
+  Run run;
+  if (!find_run<BM, TK, THREADS>(p, w, run)) return;
+
+  uint32_t voff[block_dmas<D>()];
+  block_offsets<D>(voff);
+  const uint32_t ring0 = __builtin_amdgcn_readfirstlane(lds_addr_of(lds)) + wave * (RING * ITEM);
+  const char* ring = lds + wave * (RING * ITEM);
+  constexpr int64_t STRIDE = (int64_t)BM * (D + 2);
+
+  int r = run.r;
+  int kvh = (int)(run.off / run.head_cost);
+  int64_t toff = run.off - kvh * run.head_cost;
+  int j = 0;
+  bool found = false;
+  int64_t x = run.x;
+  for (; r < p.requests; r++) {
+    const Request q = request_of(p, r);
+    const int all = q.n * p.group, tiles = (all + BM - 1) / BM;
+    if (tiles == 0) continue;
+    for (; kvh < p.n_kv; kvh++) {
+      Tiles<BM, TK> walk(q, p.group);
+      for (j = 0; j < tiles; j++) {
+        const int units = walk.next(), cost = units + AP_START;
+        if (!found) {                         // the run's first tile
+          if (toff >= cost) {
+            toff -= cost;
+            continue;
+          }
+          found = true;
+        }
+        const int64_t left = run.hi - x;
+        if (left <= 0) return;
+        const int seg = (int)(toff + left < cost ? toff + left : cost);
+        const int ua = (int)toff > AP_START ? (int)toff - AP_START : 0, ub = seg > AP_START ? seg - AP_START : 0;
+        const int64_t tile_x = x - toff;
+        const int rows = all - j * BM < BM ? all - j * BM : BM;
+        const bool begins = toff == 0;
+        x += seg - toff;
+        toff = 0;
+        if (units == 0) {                     // rows that see nothing
+          if (begins)
+            for (int idx = tid; idx < rows * D; idx += THREADS) out_row<D>(p, q, kvh, j * BM + idx / D)[idx % D] = 0;
+          continue;
+        }
+        if (ua >= ub) continue;
+        const int first = wg_of(run, tile_x + AP_START), last = wg_of(run, tile_x + cost - 1);
+
+        // ---- this wave's units of [ua, ub) ----
+        const int n_my = ub - ua > wave ? (ub - ua - wave + WAVES - 1) / WAVES : 0, n_items = 2 * n_my;
+        Wave<D, F16, RB, 1> st;
+        st.start(p, q, kvh, j * BM, all);
+        int pg[2];
+        auto fetch_pages = [&](int i) {
+          const int tok = (ua + wave + WAVES * i) * TK;
+          pg[0] = page_at(p, r, q.kv, tok);
+          pg[1] = page_at(p, r, q.kv, tok + AP_PAGE_MIN);
+        };
+        auto issue = [&](int it) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the slot's earlier contents have been read
+          const int tok = (ua + wave + WAVES * (it >> 1)) * TK;
+          const uint32_t slot = ring0 + (it % RING) * ITEM;
+#pragma unroll
+          for (int b = 0; b < 2; b++) {
+            int tokens;
+            const int64_t at = block_at<D>(p, pg[b], kvh, q.kv, tok + AP_PAGE_MIN * b, tokens);
+            dma_block<D>((it & 1) ? p.v : p.k, at, tokens, slot + b * (ITEM / 2), voff);
+          }
+          if ((it & 1) && it + 1 < n_items) fetch_pages((it + 1) >> 1);
+        };
+        auto wait_item = [&](int it) {
+          const int after = n_items - 1 - it;
+          if (after >= AHEAD) wait_vm_at_most<AHEAD * DMAS>();
+          else if (AHEAD > 2 && after == 2) wait_vm_at_most<2 * DMAS>();
+          else if (AHEAD > 1 && after == 1) wait_vm_at_most<DMAS>();
+          else wait_vm_at_most<0>();
+        };
+        static_assert(AHEAD <= 3, "wait_item");
+        if (n_my > 0) fetch_pages(0);
+#pragma unroll
+        for (int it = 0; it < AHEAD; it++)
+          if (it < n_items) issue(it);
+        const int lim0 = q.kv - q.n + (j * BM) / p.group + 1;   // what the tile's first row sees
+        for (int i = 0; i < n_my; i++) {
+          const int tok = (ua + wave + WAVES * i) * TK;
+          if (2 * i + AHEAD < n_items) issue(2 * i + AHEAD);
+          wait_item(2 * i);
+          st.scores(ring + ((2 * i) % RING) * ITEM, tok, tok + TK > lim0, p.scale_log2e);
+          if (2 * i + 1 + AHEAD < n_items) issue(2 * i + 1 + AHEAD);
+          wait_item(2 * i + 1);
+          st.values(ring + ((2 * i + 1) % RING) * ITEM);
+        }
+
+        // ---- the waves' results, a row block at a time ----
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) {
+          if (32 * rb >= rows) break;
+          __syncthreads();                    // all units read / the previous block taken
+          st.to_lds(rb, reinterpret_cast<float*>(lds + wave * (RING * ITEM)), ml[wave]);
+          __syncthreads();
+          const int here = rows - 32 * rb < 32 ? rows - 32 * rb : 32;
+          for (int idx = tid; idx < here * D; idx += THREADS) {
+            const int row = idx / D, d = idx % D;
+            float mstar = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < WAVES; i++) mstar = fmaxf(mstar, ml[i][2 * row]);
+            float acc = 0.0f, sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < WAVES; i++) {
+              const float f = part_scale(ml[i][2 * row], mstar, p.scale_log2e);
+              acc += reinterpret_cast<const float*>(lds + i * (RING * ITEM))[row * (D + 4) + d] * f;
+              sum += ml[i][2 * row + 1] * f;
+            }
+            if (first == last) {
+              out_row<D>(p, q, kvh, j * BM + 32 * rb + row)[d] = X::to_bits(sum == 0.0f ? 0.0f : acc / sum);
+            } else {
+              float* dst = p.part + slot_of(w, first) * STRIDE;
+              ap_store(dst + (32 * rb + row) * D + d, acc);
+              if (d == 0) {
+                ap_store(dst + BM * D + 2 * (32 * rb + row), mstar);
+                ap_store(dst + BM * D + 2 * (32 * rb + row) + 1, sum);
+              }
+            }
+          }
+        }
+        if (first != last) merge_if_last<D, F16, BM, THREADS>(p, q, kvh, j, rows, first, last);
+        __syncthreads();                      // the merge area becomes the rings again
+      }
+    }
+    kvh = 0;
+  }
+}
+
+// ---- wide tiles: the waves share the units --------------------------------------------------------------
+template <int D, bool F16>
+__global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs p) {
+  using X = X16<F16>;
+  constexpr int TK = 64, WAVES = 4, BM = 32 * WAVES, THREADS = 256;
+  constexpr int HALF = TK * D * 2, STAGE = 2 * HALF;     // keys, then values of one unit
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+  __shared__ float ml[WAVES][64];
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // neighbouring runs share keys and values: keep them on one XCD (workgroups go round robin over the eight)
+  const int w = (blockIdx.x & 7) * (p.wgs >> 3) + (blockIdx.x >> 3);
+  Run run;
+  if (!find_run<BM, TK, THREADS>(p, w, run)) return;
+
+  uint32_t voff[block_dmas<D>()];
+  block_offsets<D>(voff);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr_of(lds)) + wave * (AP_PAGE_MIN * D * 2);
+  constexpr int64_t STRIDE = (int64_t)BM * (D + 2);
+
+  int r = run.r;
+  int kvh = (int)(run.off / run.head_cost);
+  int64_t toff = run.off - kvh * run.head_cost;
+  bool found = false;
+  int64_t x = run.x;
+  for (; r < p.requests; r++) {
+    const Request q = request_of(p, r);
+    const int all = q.n * p.group, tiles = (all + BM - 1) / BM;
+    if (tiles == 0) continue;
+    for (; kvh < p.n_kv; kvh++) {
+      Tiles<BM, TK> walk(q, p.group);
+      for (int j = 0; j < tiles; j++) {
+        const int units = walk.next(), cost = units + AP_START;
+        if (!found) {
+          if (toff >= cost) {
+            toff -= cost;
+            continue;
+          }
+          found = true;
+        }
+        const int64_t left = run.hi - x;
+        if (left <= 0) return;
+        const int seg = (int)(toff + left < cost ? toff + left : cost);
+        const int ua = (int)toff > AP_START ? (int)toff - AP_START : 0, ub = seg > AP_START ? seg - AP_START : 0;
+        const int64_t tile_x = x - toff;
+        const int rows = all - j * BM < BM ? all - j * BM : BM;
+        const bool begins = toff == 0;
+        x += seg - toff;
+        toff = 0;
+        if (units == 0) {
+          if (begins)
+            for (int idx = tid; idx < rows * D; idx += THREADS) out_row<D>(p, q, kvh, j * BM + idx / D)[idx % D] = 0;
+          continue;
+        }
+        if (ua >= ub) continue;
+        const int first = wg_of(run, tile_x + AP_START), last = wg_of(run, tile_x + cost - 1);
+
+        const int row0 = 32 * wave;
+        const bool active = row0 < rows;
+        Wave<D, F16, 1, 2> st;
+        st.start(p, q, kvh, j * BM + row0, all);
+        // tokens seen by the wave's first and last row
+        const int last_row = j * BM + (row0 + 31 < rows ? row0 + 31 : rows - 1);
+        const int lim0 = q.kv - q.n + (j * BM + row0) / p.group + 1, lim1 = q.kv - q.n + last_row / p.group + 1;
+        int page = page_at(p, r, q.kv, ua * TK + wave * AP_PAGE_MIN);
+        auto issue = [&](int u) {
+          const int tok = u * TK + wave * AP_PAGE_MIN;
+          int tokens;
+          const int64_t at = block_at<D>(p, page, kvh, q.kv, tok, tokens);
+          const uint32_t dst = lds0 + (u & 1) * STAGE;
+          dma_block<D>(p.k, at, tokens, dst, voff);
+          dma_block<D>(p.v, at, tokens, dst + HALF, voff);
+          if (u + 1 < ub) page = page_at(p, r, q.kv, tok + TK);
+        };
+        issue(ua);
+        for (int u = ua; u < ub; u++) {
+          wait_vm_at_most<0>();
+          __syncthreads();                    // unit u has arrived, unit u - 1 has been read by all
+          if (u + 1 < ub) issue(u + 1);
+          if (active && u * TK < lim1) {
+            const char* base = lds + (u & 1) * STAGE;
+            st.scores(base, u * TK, u * TK + TK > lim0, p.scale_log2e);
+            st.values(base + HALF);
+          }
+        }
+        __syncthreads();
+
+        if (first == last) {
+          const int lane = tid & 63, c = lane & 31, h = lane >> 5;
+          const float sum = st.l[0] + __shfl_xor(st.l[0], 32, 64);
+          if (row0 + c < rows) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            uint16_t* dst = out_row<D>(p, q, kvh, j * BM + row0 + c);
+#pragma unroll
+            for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                const f32x16_t& o = st.o[0][dt];
+                *reinterpret_cast<u32x2_t*>(dst + 32 * dt + 8 * i + 4 * h) =
+                    u32x2_t{X::pack2(o[4 * i] * inv, o[4 * i + 1] * inv), X::pack2(o[4 * i + 2] * inv, o[4 * i + 3] * inv)};
+              }
+          }
+        } else {
+          // through LDS, a wave at a time in its own 64 / 4 KiB, for stores of whole lines
+          float* dst = p.part + slot_of(w, first) * STRIDE;
+          const int lane = tid & 63;
+#pragma unroll
+          for (int dt = 0; dt < D / 32; dt++) {
+            // [32 rows][32 dims + 4] of one dim block
+            float* mine = reinterpret_cast<float*>(lds + wave * 8192);
+            const int c = lane & 31, h = lane >> 5;
+            wave_lds_sync();
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const f32x16_t& o = st.o[0][dt];
+              *reinterpret_cast<f32x4_t*>(mine + c * 36 + 8 * i + 4 * h) = f32x4_t{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]};
+            }
+            wave_lds_sync();
+            for (int i = lane; i < 32 * 32; i += 64) {
+              const int row = i >> 5, d = i & 31;
+              if (row0 + row < rows) ap_store(dst + (row0 + row) * D + 32 * dt + d, mine[row * 36 + d]);
+            }
+          }
+          const float sum = st.l[0] + __shfl_xor(st.l[0], 32, 64);
+          if (lane < 32 && row0 + lane < rows) {
+            ap_store(dst + BM * D + 2 * (row0 + lane), st.m[0]);
+            ap_store(dst + BM * D + 2 * (row0 + lane) + 1, sum);
+          }
+          merge_if_last<D, F16, BM, THREADS>(p, q, kvh, j, rows, first, last);
+        }
+        __syncthreads();
+      }
+    }
+    kvh = 0;
+  }
+}
+
+constexpr int NARROW_WGS = 256;      // one per CU: 128 KiB of LDS each
+constexpr int WIDE_WGS = 512;        // two per CU: 64 KiB each
+
+template <int D, bool F16>
+void launch(const PagedArgs& base, int rows, hipStream_t s) {
+  PagedArgs a = base;
+  if (rows <= 32) {
+    a.wgs = NARROW_WGS;
+    a.min_units = 8;
+    hipLaunchKernelGGL((attn_paged_narrow_kernel<D, F16, 1, 4, 4>), dim3(a.wgs), dim3(256), 0, s, a);
+  } else if (rows <= 64) {
+    a.wgs = NARROW_WGS;
+    a.min_units = 8;
+    hipLaunchKernelGGL((attn_paged_narrow_kernel<D, F16, 2, 4, 4>), dim3(a.wgs), dim3(256), 0, s, a);
+  } else {
+    a.wgs = WIDE_WGS;
+    a.min_units = 4;
+    hipLaunchKernelGGL((attn_paged_wide_kernel<D, F16>), dim3(a.wgs), dim3(256), 0, s, a);
+  }
+}
+
+}  // namespace
+
+extern "C" int64_t mtp_attn_paged_workspace_bytes(void) {
+  return AP_COUNTER_BYTES + 2ll * WIDE_WGS * 128 * (128 + 2) * (int64_t)sizeof(float);
+}
+
+extern "C" int mtp_attn_paged(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables,
+                              const int64_t* cu, const int64_t* kv_lens, void* out, void* workspace,
+                              int64_t workspace_bytes, int64_t T, int64_t requests, int n_q_heads, int n_kv_heads,
+                              int head_dim, int64_t n_pages, int64_t page_size, int64_t max_pages, int64_t max_new,
+                              int64_t len_bound, float scale, int dtype, void* stream) {
+  MTP_REQUIRE(dtype == MTP_BF16 || dtype == MTP_F16, MTP_EUNSUPPORTED, "attn_paged: dtype %d (bf16 or f16)", dtype);
+  MTP_REQUIRE(head_dim == 64 || head_dim == 128, MTP_EUNSUPPORTED, "attn_paged: head_dim %d (64 or 128)", head_dim);
+  MTP_REQUIRE(n_q_heads > 0 && n_kv_heads > 0 && n_q_heads % n_kv_heads == 0 && n_q_heads <= 4096, MTP_EINVAL,
+              "attn_paged: heads %d/%d", n_q_heads, n_kv_heads);
+  MTP_REQUIRE(T >= 0 && T * n_q_heads <= 0x3fffffffll && requests >= 0 && requests <= 0x7fffff, MTP_EINVAL,
+              "attn_paged: T=%lld requests=%lld", (long long)T, (long long)requests);
+  MTP_REQUIRE(page_size >= AP_PAGE_MIN && (page_size & (page_size - 1)) == 0, MTP_EUNSUPPORTED,
+              "attn_paged: page_size=%lld (a power of two, at least %d)", (long long)page_size, AP_PAGE_MIN);
+  MTP_REQUIRE(n_pages > 0 && n_pages <= 0x7fffffffll && max_pages > 0 && page_size <= 0x40000000ll &&
+                  max_pages <= 0x7fffffffll / page_size,
+              MTP_EINVAL, "attn_paged: %lld pages of %lld, %lld a row", (long long)n_pages, (long long)page_size,
+              (long long)max_pages);
+  MTP_REQUIRE(max_new >= 0 && len_bound >= 0, MTP_EINVAL, "attn_paged: max_new=%lld len_bound=%lld", (long long)max_new,
+              (long long)len_bound);
+  MTP_REQUIRE(scale > 0.0f && scale < INFINITY, MTP_EINVAL, "attn_paged: scale %g", (double)scale);
+  if (T == 0 || requests == 0) return MTP_OK;
+  MTP_REQUIRE(q && k_cache && v_cache && block_tables && cu && kv_lens && out, MTP_EINVAL, "attn_paged: null pointer");
+  MTP_REQUIRE(((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)workspace) % 16 == 0,
+              MTP_EINVAL, "attn_paged: tensors must be 16-byte aligned");
+  MTP_REQUIRE(workspace && workspace_bytes >= mtp_attn_paged_workspace_bytes(), MTP_EWORKSPACE,
+              "attn_paged: workspace %lld bytes, need %lld", (long long)workspace_bytes,
+              (long long)mtp_attn_paged_workspace_bytes());
+  PagedArgs a = {};
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k_cache);
+  a.v = static_cast<const uint16_t*>(v_cache);
+  a.table = block_tables;
+  a.cu = cu;
+  a.kv_lens = kv_lens;
+  a.out = static_cast<uint16_t*>(out);
+  a.arrived = static_cast<int32_t*>(workspace);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + AP_COUNTER_BYTES);
+  a.max_pages = max_pages;
+  a.T = (int)T;
+  a.requests = (int)requests;
+  a.n_q = n_q_heads;
+  a.n_kv = n_kv_heads;
+  a.group = n_q_heads / n_kv_heads;
+  a.page_shift = __builtin_ctzll((unsigned long long)page_size);
+  a.n_pages = (int)n_pages;
+  a.room = (int)(max_pages * page_size);
+  a.scale_log2e = scale * 1.4426950408889634f;
+  const int64_t most = (max_new < T ? max_new : T) * a.group;
+  const int rows = most > 1 << 20 ? 1 << 20 : (int)most;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool f16 = dtype == MTP_F16;
+  if (head_dim == 64) {
+    if (f16) launch<64, true>(a, rows, s);
+    else launch<64, false>(a, rows, s);
+  } else {
+    if (f16) launch<128, true>(a, rows, s);
+    else launch<128, false>(a, rows, s);
+  }
+  MTP_CHECK_LAUNCH("attn_paged");
+  return MTP_OK;
+}

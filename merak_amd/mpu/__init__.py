@@ -24,6 +24,8 @@ from .random import get_rng_tracker
 from .random import model_parallel_manual_seed
 from .random import RNGStatesTracker
 
+from .rotary import qk_norm_rotary
+
 from .utils import divide
 from .utils import ensure_divisibility
 from .utils import split_tensor_along_last_dim

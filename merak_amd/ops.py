@@ -8,7 +8,7 @@ there is no fallback path.
 from __future__ import annotations
 
 import threading
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -693,3 +693,277 @@ def attn_decode_append(qkv: torch.Tensor, cos_table: torch.Tensor, sin_table: to
                                                      cos_table.shape[0], len_bound, scale, _dt(qkv), _stream(dev)),
                    "mtp_attn_decode_append")
     return out
+
+
+# --------------------------------------------------------------------------- paged key/value cache
+class PagedPlan(NamedTuple):
+    """What ``paged_plan`` hands out for one step (all on the device)."""
+    slots: torch.Tensor        # int64 [tokens]: cache slot of each new token, -1: none
+    positions: torch.Tensor    # int64 [tokens]: its position in its request, -1: none
+    cu: torch.Tensor           # int64 [requests + 1]: where each request's tokens start
+    kv_lens: torch.Tensor      # int64 [requests]: tokens cached after the step, 0 for a refused request
+    granted: torch.Tensor      # bool [requests]: False: refused, nothing of it has changed
+    held: torch.Tensor         # int32 [requests]: pages each request holds after the step
+    free_count: torch.Tensor   # int32 [1]: pages left on the free list
+
+
+def _index(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape: Tuple[int, ...]) -> torch.Tensor:
+    if t.dtype != dtype or tuple(t.shape) != shape:
+        raise ValueError(f"{what}: {name} must be {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
+    return _contig(t)
+
+
+def _own(what: str, name: str, t: torch.Tensor) -> torch.Tensor:
+    """A tensor that the call writes into: it must be the caller's memory as it is."""
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: {name} is written in place and must be contiguous")
+    return t
+
+
+def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """Contiguous and on a 16-byte boundary (a slice of a larger tensor may start anywhere)."""
+    if t is None:
+        return None
+    t = _contig(t)
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def paged_plan(lens: torch.Tensor, new_lens: torch.Tensor, held: torch.Tensor, block_tables: torch.Tensor,
+               free_pages: torch.Tensor, free_count: torch.Tensor, page_size: int, tokens: int) -> PagedPlan:
+    """Pages, slots and positions of the ``new_lens[r]`` tokens that arrive for each request, one launch.
+
+    ``block_tables`` int32 [requests, max_pages] gets the new pages behind the ``held[r]`` ones (in place); they come
+    from the top of ``free_pages`` int32, of which ``free_count`` int32 [1] are free.  ``tokens``: length of the
+    per-token outputs, at least the new tokens of all requests.  The caller goes on with the returned ``held`` and
+    ``free_count``, and with ``lens + new_lens`` where ``granted``."""
+    dev = _require_gpu(lens, new_lens, held, block_tables, free_pages, free_count)
+    if block_tables.dim() != 2 or block_tables.dtype != torch.int32:
+        raise ValueError("paged_plan: block_tables must be int32 [requests, max_pages]")
+    R, max_pages = block_tables.shape
+    lens = _index("paged_plan", "lens", lens, torch.int64, (R,))
+    new_lens = _index("paged_plan", "new_lens", new_lens, torch.int64, (R,))
+    held = _index("paged_plan", "held", held, torch.int32, (R,))
+    free_pages = _index("paged_plan", "free_pages", free_pages, torch.int32, (free_pages.numel(),))
+    free_count = _index("paged_plan", "free_count", free_count, torch.int32, (1,))
+    _own("paged_plan", "block_tables", block_tables)
+    tokens = int(tokens)
+    if tokens < 0:
+        raise ValueError(f"paged_plan: tokens={tokens}")
+    i64 = lambda n: torch.empty((n,), dtype=torch.int64, device=dev)
+    plan = PagedPlan(i64(tokens), i64(tokens), i64(R + 1), i64(R), torch.empty((R,), dtype=torch.bool, device=dev),
+                     torch.empty_like(held), torch.empty_like(free_count))
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().mtp_paged_plan(_p(lens), _p(new_lens), _p(held), _p(block_tables), _p(free_pages),
+                                             _p(free_count), _p(plan.slots), _p(plan.positions), _p(plan.cu),
+                                             _p(plan.kv_lens), _p(plan.granted), _p(plan.held), _p(plan.free_count), R,
+                                             max_pages, int(page_size), free_pages.numel(), tokens, _stream(dev)),
+                   "mtp_paged_plan")
+    return plan
+
+
+def paged_release(finished: torch.Tensor, held: torch.Tensor, block_tables: torch.Tensor, free_pages: torch.Tensor,
+                  free_count: torch.Tensor) -> None:
+    """Pages of the requests with ``finished[r]`` (bool [requests]) go back on the free list; ``held``, ``free_pages``
+    and ``free_count`` are updated in place."""
+    dev = _require_gpu(finished, held, block_tables, free_pages, free_count)
+    if block_tables.dim() != 2 or block_tables.dtype != torch.int32:
+        raise ValueError("paged_release: block_tables must be int32 [requests, max_pages]")
+    R, max_pages = block_tables.shape
+    finished = _index("paged_release", "finished", finished, torch.bool, (R,))
+    for name, t, n in (("held", held, R), ("free_pages", free_pages, free_pages.numel()), ("free_count", free_count, 1)):
+        _index("paged_release", name, _own("paged_release", name, t), torch.int32, (n,))
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().mtp_paged_release(_p(finished), _p(held), _p(_contig(block_tables)), _p(free_pages),
+                                                _p(free_count), R, max_pages, free_pages.numel(), _stream(dev)),
+                   "mtp_paged_release")
+
+
+def _rotary_args(what: str, qkv, cos_table, sin_table, positions, n_q_heads, n_kv_heads, q_weight, k_weight):
+    """Checks shared by the three forms -> (qkv, cos, sin, positions, q_weight, k_weight, T, head_dim)."""
+    if cos_table.dim() != 2 or cos_table.shape != sin_table.shape or cos_table.dtype != sin_table.dtype:
+        raise ValueError(f"{what}: cos / sin tables must be [max_positions, head_dim] of one type")
+    hd = cos_table.shape[1]
+    if cos_table.dtype not in (torch.float32, qkv.dtype):
+        raise TypeError(f"{what}: tables must be float32 or of the type of qkv, got {cos_table.dtype}")
+    if qkv.dim() != 2 or n_q_heads <= 0 or n_kv_heads <= 0 or qkv.shape[1] != (n_q_heads + 2 * n_kv_heads) * hd:
+        raise ValueError(f"{what}: qkv {tuple(qkv.shape)} for {n_q_heads}+2*{n_kv_heads} heads of {hd}")
+    T = qkv.shape[0]
+    positions = _index(what, "positions", positions, torch.int64, (T,))
+    for w in (q_weight, k_weight):
+        if w is not None and (w.shape != (hd,) or w.dtype != qkv.dtype):
+            raise ValueError(f"{what}: norm weight {tuple(w.shape)} {w.dtype} for heads of {hd} {qkv.dtype}")
+    return (_aligned(qkv), _aligned(cos_table), _aligned(sin_table), positions, _aligned(q_weight), _aligned(k_weight), T,
+            hd)
+
+
+def _kv_heads(what: str, qkv: torch.Tensor, cos_table: torch.Tensor, n_q_heads: int) -> int:
+    if qkv.dim() != 2 or cos_table.dim() != 2 or cos_table.shape[1] == 0:
+        raise ValueError(f"{what}: qkv must be [T, heads * head_dim] and the tables [max_positions, head_dim]")
+    rest = qkv.shape[1] // cos_table.shape[1] - n_q_heads
+    if rest <= 0 or rest % 2:
+        raise ValueError(f"{what}: qkv {tuple(qkv.shape)} is not {n_q_heads} query heads and as many key as value heads of "
+                         f"{cos_table.shape[1]}")
+    return rest // 2
+
+
+def qk_norm_rope(qkv: torch.Tensor, cos_table: torch.Tensor, sin_table: torch.Tensor, positions: torch.Tensor,
+                 n_q_heads: int, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                 eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """-> (q [T, n_q, head_dim], k [T, n_kv, head_dim]): RMSNorm of each query and key head of ``qkv``
+    [T, (n_q + 2 n_kv) * head_dim] with ``q_weight`` / ``k_weight`` [head_dim] (None: no norm), then the rotary embedding
+    at ``positions`` int64 [T].  fp32 inside, rounded once.  ``mpu.qk_norm_rotary`` is the form with a gradient."""
+    dev = _require_gpu(qkv, cos_table, sin_table, positions, q_weight, k_weight)
+    n_kv = _kv_heads("qk_norm_rope", qkv, cos_table, n_q_heads)
+    qkv, cos, sin, positions, qw, kw, T, hd = _rotary_args("qk_norm_rope", qkv, cos_table, sin_table, positions, n_q_heads,
+                                                           n_kv, q_weight, k_weight)
+    q = torch.empty((T, n_q_heads, hd), dtype=qkv.dtype, device=dev)
+    k = torch.empty((T, n_kv, hd), dtype=qkv.dtype, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().mtp_qk_norm_rope(_p(qkv), _p(cos), _p(sin), _dt(cos), _p(positions), _p(qw), _p(kw), _p(q),
+                                               _p(k), T, n_q_heads, n_kv, hd, cos.shape[0], float(eps), _dt(qkv),
+                                               _stream(dev)), "mtp_qk_norm_rope")
+    return q, k
+
+
+def qk_norm_rope_bwd(dq: Optional[torch.Tensor], dk: Optional[torch.Tensor], dv: Optional[torch.Tensor], qkv: torch.Tensor,
+                     cos_table: torch.Tensor, sin_table: torch.Tensor, positions: torch.Tensor,
+                     q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                     n_q_heads: Optional[int] = None, want_dw: bool = True):
+    """-> (dqkv, dq_weight or None, dk_weight or None).  ``dq`` [T, n_q, head_dim], ``dk`` and ``dv`` [T, n_kv, head_dim]
+    (None: no gradient); ``dv`` is copied into the values' place of ``dqkv``.  ``n_q_heads`` is needed without ``dq``."""
+    dev = _require_gpu(qkv, dq, dk, dv, cos_table, sin_table, positions, q_weight, k_weight)
+    if n_q_heads is None:
+        if dq is None or dq.dim() != 3:
+            raise ValueError("qk_norm_rope_bwd: n_q_heads is needed without dq [T, n_q, head_dim]")
+        n_q_heads = dq.shape[1]
+    n_kv = _kv_heads("qk_norm_rope_bwd", qkv, cos_table, n_q_heads)
+    qkv, cos, sin, positions, qw, kw, T, hd = _rotary_args("qk_norm_rope_bwd", qkv, cos_table, sin_table, positions,
+                                                           n_q_heads, n_kv, q_weight, k_weight)
+    for name, g, n in (("dq", dq, n_q_heads), ("dk", dk, n_kv), ("dv", dv, n_kv)):
+        if g is not None and (g.shape != (T, n, hd) or g.dtype != qkv.dtype):
+            raise ValueError(f"qk_norm_rope_bwd: {name} must be {qkv.dtype} {[T, n, hd]}, got {g.dtype} {list(g.shape)}")
+    dq, dk, dv = _aligned(dq), _aligned(dk), _aligned(dv)
+    dqkv = torch.empty_like(qkv)
+    dqw = torch.empty_like(qw) if want_dw and qw is not None else None
+    dkw = torch.empty_like(kw) if want_dw and kw is not None else None
+    if T == 0:
+        return dqkv, None if dqw is None else dqw.zero_(), None if dkw is None else dkw.zero_()
+    lib = _lib.lib()
+    ws = None
+    if dqw is not None or dkw is not None:
+        need = lib.mtp_qk_norm_rope_bwd_workspace_bytes(T, n_q_heads, n_kv, hd)
+        ws = torch.empty((max(int(need), 4),), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(lib.mtp_qk_norm_rope_bwd(_p(dq), _p(dk), _p(dv), _p(qkv), _p(cos), _p(sin), _dt(cos), _p(positions),
+                                            _p(qw), _p(kw), _p(dqkv), _p(dqw), _p(dkw), _p(ws),
+                                            0 if ws is None else ws.numel(), T, n_q_heads, n_kv, hd, cos.shape[0],
+                                            float(eps), _dt(qkv), _stream(dev)), "mtp_qk_norm_rope_bwd")
+    return dqkv, dqw, dkw
+
+
+def _pages(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor):
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError(f"{what}: caches must be contiguous [n_pages, n_kv_heads, page_size, head_dim] of one shape")
+    return k_cache.shape
+
+
+def qk_norm_rope_append(qkv: torch.Tensor, cos_table: torch.Tensor, sin_table: torch.Tensor, positions: torch.Tensor,
+                        slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_q_heads: int,
+                        q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                        eps: float = 1e-6) -> torch.Tensor:
+    """``qk_norm_rope`` for serving: returns q [T, n_q, head_dim] and writes the keys and the values of each row to
+    ``slots[t]`` of the caches [n_pages, n_kv, page_size, head_dim] (-1: nowhere)."""
+    dev = _require_gpu(qkv, cos_table, sin_table, positions, slots, k_cache, v_cache, q_weight, k_weight)
+    n_pages, n_kv, page_size, hd = _pages("qk_norm_rope_append", k_cache, v_cache)
+    if cos_table.dim() != 2 or cos_table.shape[1] != hd or k_cache.dtype != qkv.dtype or v_cache.dtype != qkv.dtype:
+        raise ValueError("qk_norm_rope_append: caches and tables must match the heads and the type of qkv")
+    qkv, cos, sin, positions, qw, kw, T, hd = _rotary_args("qk_norm_rope_append", qkv, cos_table, sin_table, positions,
+                                                           n_q_heads, n_kv, q_weight, k_weight)
+    slots = _index("qk_norm_rope_append", "slots", slots, torch.int64, (T,))
+    q = torch.empty((T, n_q_heads, hd), dtype=qkv.dtype, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().mtp_qk_norm_rope_append(_p(qkv), _p(cos), _p(sin), _dt(cos), _p(positions), _p(slots), _p(qw),
+                                                      _p(kw), _p(q), _p(k_cache), _p(v_cache), T, n_q_heads, n_kv, hd,
+                                                      cos.shape[0], n_pages, page_size, float(eps), _dt(qkv),
+                                                      _stream(dev)), "mtp_qk_norm_rope_append")
+    return q
+
+
+def attn_paged_workspace(device) -> torch.Tensor:
+    """Scratch for ``attn_paged``, any shape (the kernels need its head zero before the first use and leave it zero).
+    Launches that may overlap in time need one each."""
+    ws = torch.empty((int(_lib.lib().mtp_attn_paged_workspace_bytes()),), dtype=torch.uint8, device=device)
+    ws[:4096].zero_()
+    return ws
+
+
+def attn_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+               cu: torch.Tensor, kv_lens: torch.Tensor, scale: Optional[float] = None, max_new: Optional[int] = None,
+               len_bound: Optional[int] = None, workspace: Optional[torch.Tensor] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal grouped-query attention of each request's new tokens over its pages, any mix of single tokens, drafts and
+    prompts.  q [T, n_q, head_dim]; rows cu[r] .. cu[r+1]-1 are request r's, whose last one is token kv_lens[r] - 1 of
+    the pages that row r of ``block_tables`` names.  ``max_new`` / ``len_bound``: upper bounds of a request's new tokens
+    and of kv_lens known on the host (they choose how the work is laid out).  Rows of no request are left as they were in
+    ``out`` (unspecified in a new tensor).  ``workspace``: from ``attn_paged_workspace``."""
+    dev = _require_gpu(q, k_cache, v_cache, block_tables, cu, kv_lens, workspace, out)
+    n_pages, n_kv, page_size, hd = _pages("attn_paged", k_cache, v_cache)
+    if q.dim() != 3 or q.shape[2] != hd or q.shape[1] % n_kv or q.shape[1] == 0:
+        raise ValueError(f"attn_paged: q {tuple(q.shape)} against caches {tuple(k_cache.shape)}")
+    if not (q.dtype == k_cache.dtype == v_cache.dtype):
+        raise ValueError("attn_paged: q and the caches must share a dtype")
+    if block_tables.dim() != 2 or block_tables.dtype != torch.int32:
+        raise ValueError("attn_paged: block_tables must be int32 [requests, max_pages]")
+    R, max_pages = block_tables.shape
+    cu = _index("attn_paged", "cu", cu, torch.int64, (R + 1,))
+    kv_lens = _index("attn_paged", "kv_lens", kv_lens, torch.int64, (R,))
+    q, block_tables = _aligned(q), _contig(block_tables)
+    T, n_q = q.shape[:2]
+    max_new = T if max_new is None else int(max_new)
+    len_bound = max_pages * page_size if len_bound is None else int(len_bound)
+    scale = hd ** -0.5 if scale is None else float(scale)
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError("attn_paged: out must be a contiguous, 16-byte aligned tensor like q")
+    if workspace is None:
+        workspace = attn_paged_workspace(dev)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().mtp_attn_paged(_p(q), _p(k_cache), _p(v_cache), _p(block_tables), _p(cu), _p(kv_lens), _p(out),
+                                             _p(workspace), workspace.numel() * workspace.element_size(), T, R, n_q, n_kv,
+                                             hd, n_pages, page_size, max_pages, max_new, len_bound, scale, _dt(q),
+                                             _stream(dev)), "mtp_attn_paged")
+    return out
+
+
+def verify_draft(draft_tokens: torch.Tensor, target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor],
+                 uniforms: torch.Tensor, draft_lens: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """-> (tokens int64 [R, K + 1], accepted int64 [R]): the accepted drafts of each request, the token drawn after them,
+    then -1.  ``draft_tokens`` int64 [R, K]; ``target_probs`` [R, K + 1, V]; ``draft_probs`` [R, K, V] of the same type,
+    or None where the drafts were certain; ``uniforms`` fp32 [R, K + 1] in [0, 1): one per draft, the last for the drawn
+    token; ``draft_lens`` int64 [R] limits the drafts of a request."""
+    dev = _require_gpu(draft_tokens, target_probs, draft_probs, uniforms, draft_lens)
+    if draft_tokens.dim() != 2 or target_probs.dim() != 3:
+        raise ValueError("verify_draft: draft_tokens must be [R, K] and target_probs [R, K + 1, V]")
+    R, K = draft_tokens.shape
+    V = target_probs.shape[2]
+    draft_tokens = _index("verify_draft", "draft_tokens", draft_tokens, torch.int64, (R, K))
+    uniforms = _index("verify_draft", "uniforms", uniforms, torch.float32, (R, K + 1))
+    if target_probs.shape != (R, K + 1, V):
+        raise ValueError(f"verify_draft: target_probs {tuple(target_probs.shape)} for {R} requests of {K} drafts")
+    if draft_probs is not None and (draft_probs.shape != (R, K, V) or draft_probs.dtype != target_probs.dtype):
+        raise ValueError("verify_draft: draft_probs must be [R, K, V] of the type of target_probs")
+    if draft_lens is not None:
+        draft_lens = _index("verify_draft", "draft_lens", draft_lens, torch.int64, (R,))
+    target_probs = _contig(target_probs)
+    draft_probs = None if draft_probs is None else _contig(draft_probs)
+    tokens = torch.empty((R, K + 1), dtype=torch.int64, device=dev)
+    accepted = torch.empty((R,), dtype=torch.int64, device=dev)
+    lib = _lib.lib()
+    need = int(lib.mtp_verify_draft_workspace_bytes(R, V))
+    ws = torch.empty((max(need, 8),), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(lib.mtp_verify_draft(_p(draft_tokens), _p(draft_lens), _p(target_probs), _p(draft_probs), _p(uniforms),
+                                        _p(tokens), _p(accepted), _p(ws), ws.numel(), R, K, V, _dt(target_probs),
+                                        _stream(dev)), "mtp_verify_draft")
+    return tokens, accepted
