@@ -66,12 +66,24 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
                    (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
 }
 
-__device__ __forceinline__ void ap_store(float* p, float v) {   // served at the level all XCDs share
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float ap_load(const float* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
+// Partial results in the workspace: accesses at device scope (sc1), served at the level all XCDs share
+struct Partials {
+  static constexpr int SC1 = 16;
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ explicit Partials(float* base) : r(__builtin_amdgcn_make_buffer_rsrc(base, 0, 0x7fffffff, 0x00020000)) {}
+  __device__ __forceinline__ void store4(int at, f32x4_t v) const {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), r, at * 4, 0, SC1);
+  }
+  __device__ __forceinline__ void store2(int at, float a, float b) const {
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(a), __float_as_uint(b)}, r, at * 4, 0, SC1);
+  }
+  __device__ __forceinline__ f32x4_t load4(int at) const {
+    return __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, at * 4, 0, SC1));
+  }
+  __device__ __forceinline__ f32x2_t load2(int at) const {
+    return __builtin_bit_cast(f32x2_t, __builtin_amdgcn_raw_buffer_load_b64(r, at * 4, 0, SC1));
+  }
+};
 
 template <int N> __device__ __forceinline__ void wait_vm_at_most() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
@@ -188,6 +200,9 @@ template <int D> __device__ __forceinline__ int swz(int t) {
   return (((t >> 1) & 3) << 1) | ((t >> 3) & 1);       // two rows share the 256 bytes of the banks
 }
 
+// place of element d of a row in the merge area
+template <int D> __device__ __forceinline__ int merge_at(int row, int d) { return row * D + (d ^ ((row & 7) << 2)); }
+
 template <int D, bool F16, int RB, int NB>
 struct Wave {
   using X = X16<F16>;
@@ -302,15 +317,21 @@ struct Wave {
     }
   }
 
-  // row block rb as fp32 [32][D + 4] (padded: rows start in different banks) and (m, l) per row
+  // four consecutive dims of the lane's row: 32 dt + 8 i + 4 h
+  __device__ __forceinline__ f32x4_t quad(int rb, int dt, int i) const {
+    return f32x4_t{o[rb][dt][4 * i], o[rb][dt][4 * i + 1], o[rb][dt][4 * i + 2], o[rb][dt][4 * i + 3]};
+  }
+
+  // row block rb as fp32 [32][D] and (m, l) per row; groups of four floats are swizzled by the row (merge_at), so that
+  // the lanes' rows fall into different banks
   __device__ __forceinline__ void to_lds(int rb, float* dst, float* ml) const {
     const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        *reinterpret_cast<f32x4_t*>(dst + row * (D + 4) + 32 * dt + 8 * i + 4 * h) =
-            f32x4_t{o[rb][dt][4 * i], o[rb][dt][4 * i + 1], o[rb][dt][4 * i + 2], o[rb][dt][4 * i + 3]};
+        *reinterpret_cast<f32x4_t*>(dst + merge_at<D>(row, 32 * dt + 8 * i + 4 * h)) =
+            quad(rb, dt, i);
     const float sum = l[rb] + __shfl_xor(l[rb], 32, 64);
     if (h == 0) {
       ml[2 * row] = m[rb];
@@ -330,13 +351,16 @@ template <int D> __device__ __forceinline__ void block_offsets(uint32_t* voff) {
     voff[j] = (uint32_t)(t * D * 2 + (((lane % CHUNKS) ^ swz<D>(t)) << 4));
   }
 }
-template <int D>
+template <int D, bool ONCE>   // ONCE: nothing else in the launch reads these rows
 __device__ __forceinline__ void dma_block(const uint16_t* cache, int64_t offset, int tokens, uint32_t lds_addr, const uint32_t* voff) {
   const rsrc_t v = make_rsrc(cache + offset, (int64_t)tokens * (D * 2));
   const rsrc_t r = {__builtin_amdgcn_readfirstlane(v[0]), __builtin_amdgcn_readfirstlane(v[1]),
                     __builtin_amdgcn_readfirstlane(v[2]), v[3]};
 #pragma unroll
-  for (int j = 0; j < block_dmas<D>(); j++) dma16(r, lds_addr + j * 1024, voff[j], 0);
+  for (int j = 0; j < block_dmas<D>(); j++) {
+    if (ONCE) dma16_nt(r, lds_addr + j * 1024, voff[j], 0);
+    else dma16(r, lds_addr + j * 1024, voff[j], 0);
+  }
 }
 
 // page of the block of 16 tokens at tok, -1 when it is unknown or the request ends before
@@ -356,7 +380,14 @@ __device__ __forceinline__ int64_t block_at(const PagedArgs& p, int page, int kv
 
 // ---- results of a tile --------------------------------------------------------------------------------
 // where partial results of a workgroup go: its first tile (started by an earlier workgroup) and its last (its own)
-__device__ __forceinline__ int64_t slot_of(int w, int first) { return 2 * (int64_t)w + (w == first ? 1 : 0); }
+__device__ __forceinline__ int slot_of(int w, int first) { return 2 * w + (w == first ? 1 : 0); }
+
+template <bool F16> __device__ __forceinline__ void store_out(uint16_t* dst, f32x4_t o, float inv) {
+  using X = X16<F16>;
+  *reinterpret_cast<u32x2_t*>(dst) = u32x2_t{X::pack2(o[0] * inv, o[1] * inv), X::pack2(o[2] * inv, o[3] * inv)};
+}
+// a sum of zero is a row that sees nothing (NaN is not: it has to be seen)
+__device__ __forceinline__ float inverse(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
 
 template <int D>
 __device__ __forceinline__ uint16_t* out_row(const PagedArgs& p, const Request& q, int kvh, int row) {
@@ -375,7 +406,6 @@ __device__ __forceinline__ float part_scale(float m, float common, float c) {
 // its stores are acknowledged, then counts itself.
 template <int D, bool F16, int BM, int THREADS>
 __device__ __forceinline__ void merge_if_last(const PagedArgs& p, const Request& q, int kvh, int tile, int rows, int first, int last) {
-  using X = X16<F16>;
   __shared__ int is_last;
   const int tid = threadIdx.x;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -387,50 +417,51 @@ __device__ __forceinline__ void merge_if_last(const PagedArgs& p, const Request&
   }
   __syncthreads();
   if (!is_last) return;
-  constexpr int64_t STRIDE = (int64_t)BM * (D + 2);
-  for (int idx = tid; idx < rows * D; idx += THREADS) {
-    const int row = idx / D, d = idx % D;
-    float mstar = -INFINITY, acc = 0.0f, sum = 0.0f;
-    for (int w0 = first; w0 <= last; w0 += 8) {
-      float mv[8], ov[8], lv[8];
+  constexpr int STRIDE = BM * (D + 2), BATCH = 8;
+  const Partials part(p.part);
+  for (int idx = tid; idx < rows * (D / 4); idx += THREADS) {
+    const int row = idx / (D / 4), d = idx % (D / 4) * 4;
+    float mstar = -INFINITY, sum = 0.0f;
+    f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int w0 = first; w0 <= last; w0 += BATCH) {
+      f32x2_t ml[BATCH];
+      f32x4_t ov[BATCH];
 #pragma unroll
-      for (int u = 0; u < 8; u++) {
-        const int w = w0 + u <= last ? w0 + u : w0;
-        const float* src = p.part + slot_of(w, first) * STRIDE;
-        mv[u] = ap_load(src + BM * D + 2 * row);
-        lv[u] = ap_load(src + BM * D + 2 * row + 1);
-        ov[u] = ap_load(src + row * D + d);
-        if (w0 + u > last) {
-          mv[u] = -INFINITY;
-          lv[u] = ov[u] = 0.0f;
-        }
+      for (int u = 0; u < BATCH; u++) {
+        const int src = slot_of(w0 + u <= last ? w0 + u : w0, first) * STRIDE;
+        ml[u] = part.load2(src + BM * D + 2 * row);
+        ov[u] = part.load4(src + row * D + d);
       }
       float mn = mstar;
 #pragma unroll
-      for (int u = 0; u < 8; u++) mn = fmaxf(mn, mv[u]);
+      for (int u = 0; u < BATCH; u++) {
+        if (w0 + u > last) {
+          ml[u] = f32x2_t{-INFINITY, 0.0f};
+          ov[u] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        mn = fmaxf(mn, ml[u][0]);
+      }
       const float keep = part_scale(mstar, mn, p.scale_log2e);
       acc *= keep;
       sum *= keep;
 #pragma unroll
-      for (int u = 0; u < 8; u++) {
-        const float f = part_scale(mv[u], mn, p.scale_log2e);
+      for (int u = 0; u < BATCH; u++) {
+        const float f = part_scale(ml[u][0], mn, p.scale_log2e);
         acc += ov[u] * f;
-        sum += lv[u] * f;
+        sum += ml[u][1] * f;
       }
       mstar = mn;
     }
-    // a sum that is not positive is a row that sees nothing - or NaN, which has to be seen
-    out_row<D>(p, q, kvh, tile * BM + row)[d] = X::to_bits(sum == 0.0f ? 0.0f : acc / sum);
+    store_out<F16>(out_row<D>(p, q, kvh, tile * BM + row) + d, acc, inverse(sum));
   }
 }
 
 // ---- narrow tiles: the waves take turns with the units ------------------------------------------------------
 template <int D, bool F16, int RB, int WAVES, int RING>
 __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const PagedArgs p) {
-  using X = X16<F16>;
   constexpr int TK = 32, BM = 32 * RB, THREADS = WAVES * 64;
   constexpr int ITEM = TK * D * 2, DMAS = ITEM / 1024, AHEAD = RING - 1;
-  static_assert(32 * (D + 4) * 4 <= RING * ITEM && AHEAD * DMAS < 64, "merge area / vmcnt range");
+  static_assert(32 * D * 4 <= RING * ITEM && AHEAD * DMAS < 64, "merge area / vmcnt range");
   __shared__ __attribute__((aligned(1024))) char lds[WAVES * RING * ITEM];
   __shared__ float ml[WAVES][64];
   const int tid = threadIdx.x;
@@ -443,7 +474,8 @@ __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const Pag
   block_offsets<D>(voff);
   const uint32_t ring0 = __builtin_amdgcn_readfirstlane(lds_addr_of(lds)) + wave * (RING * ITEM);
   const char* ring = lds + wave * (RING * ITEM);
-  constexpr int64_t STRIDE = (int64_t)BM * (D + 2);
+  constexpr int STRIDE = BM * (D + 2);
+  const Partials part(p.part);
 
   int r = run.r;
   int kvh = (int)(run.off / run.head_cost);
@@ -485,8 +517,6 @@ __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const Pag
 
         // ---- this wave's units of [ua, ub) ----
         const int n_my = ub - ua > wave ? (ub - ua - wave + WAVES - 1) / WAVES : 0, n_items = 2 * n_my;
-        Wave<D, F16, RB, 1> st;
-        st.start(p, q, kvh, j * BM, all);
         int pg[2];
         auto fetch_pages = [&](int i) {
           const int tok = (ua + wave + WAVES * i) * TK;
@@ -501,7 +531,7 @@ __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const Pag
           for (int b = 0; b < 2; b++) {
             int tokens;
             const int64_t at = block_at<D>(p, pg[b], kvh, q.kv, tok + AP_PAGE_MIN * b, tokens);
-            dma_block<D>((it & 1) ? p.v : p.k, at, tokens, slot + b * (ITEM / 2), voff);
+            dma_block<D, true>((it & 1) ? p.v : p.k, at, tokens, slot + b * (ITEM / 2), voff);
           }
           if ((it & 1) && it + 1 < n_items) fetch_pages((it + 1) >> 1);
         };
@@ -517,6 +547,8 @@ __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const Pag
 #pragma unroll
         for (int it = 0; it < AHEAD; it++)
           if (it < n_items) issue(it);
+        Wave<D, F16, RB, 1> st;
+        st.start(p, q, kvh, j * BM, all);
         const int lim0 = q.kv - q.n + (j * BM) / p.group + 1;   // what the tile's first row sees
         for (int i = 0; i < n_my; i++) {
           const int tok = (ua + wave + WAVES * i) * TK;
@@ -536,27 +568,24 @@ __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const Pag
           st.to_lds(rb, reinterpret_cast<float*>(lds + wave * (RING * ITEM)), ml[wave]);
           __syncthreads();
           const int here = rows - 32 * rb < 32 ? rows - 32 * rb : 32;
-          for (int idx = tid; idx < here * D; idx += THREADS) {
-            const int row = idx / D, d = idx % D;
-            float mstar = -INFINITY;
+          for (int idx = tid; idx < here * (D / 4); idx += THREADS) {
+            const int row = idx / (D / 4), d = idx % (D / 4) * 4;
+            float mstar = -INFINITY, sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < WAVES; i++) mstar = fmaxf(mstar, ml[i][2 * row]);
-            float acc = 0.0f, sum = 0.0f;
+            f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < WAVES; i++) {
               const float f = part_scale(ml[i][2 * row], mstar, p.scale_log2e);
-              acc += reinterpret_cast<const float*>(lds + i * (RING * ITEM))[row * (D + 4) + d] * f;
+              acc += *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(lds + i * (RING * ITEM)) + merge_at<D>(row, d)) * f;
               sum += ml[i][2 * row + 1] * f;
             }
             if (first == last) {
-              out_row<D>(p, q, kvh, j * BM + 32 * rb + row)[d] = X::to_bits(sum == 0.0f ? 0.0f : acc / sum);
+              store_out<F16>(out_row<D>(p, q, kvh, j * BM + 32 * rb + row) + d, acc, inverse(sum));
             } else {
-              float* dst = p.part + slot_of(w, first) * STRIDE;
-              ap_store(dst + (32 * rb + row) * D + d, acc);
-              if (d == 0) {
-                ap_store(dst + BM * D + 2 * (32 * rb + row), mstar);
-                ap_store(dst + BM * D + 2 * (32 * rb + row) + 1, sum);
-              }
+              const int dst = slot_of(w, first) * STRIDE;
+              part.store4(dst + (32 * rb + row) * D + d, acc);
+              if (d == 0) part.store2(dst + BM * D + 2 * (32 * rb + row), mstar, sum);
             }
           }
         }
@@ -571,7 +600,6 @@ __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const Pag
 // ---- wide tiles: the waves share the units --------------------------------------------------------------
 template <int D, bool F16>
 __global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs p) {
-  using X = X16<F16>;
   constexpr int TK = 64, WAVES = 4, BM = 32 * WAVES, THREADS = 256;
   constexpr int HALF = TK * D * 2, STAGE = 2 * HALF;     // keys, then values of one unit
   __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
@@ -586,7 +614,8 @@ __global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs
   uint32_t voff[block_dmas<D>()];
   block_offsets<D>(voff);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr_of(lds)) + wave * (AP_PAGE_MIN * D * 2);
-  constexpr int64_t STRIDE = (int64_t)BM * (D + 2);
+  constexpr int STRIDE = BM * (D + 2);
+  const Partials part(p.part);
 
   int r = run.r;
   int kvh = (int)(run.off / run.head_cost);
@@ -638,8 +667,8 @@ __global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs
           int tokens;
           const int64_t at = block_at<D>(p, page, kvh, q.kv, tok, tokens);
           const uint32_t dst = lds0 + (u & 1) * STAGE;
-          dma_block<D>(p.k, at, tokens, dst, voff);
-          dma_block<D>(p.v, at, tokens, dst + HALF, voff);
+          dma_block<D, false>(p.k, at, tokens, dst, voff);
+          dma_block<D, false>(p.v, at, tokens, dst + HALF, voff);
           if (u + 1 < ub) page = page_at(p, r, q.kv, tok + TK);
         };
         issue(ua);
@@ -657,45 +686,34 @@ __global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs
 
         if (first == last) {
           const int lane = tid & 63, c = lane & 31, h = lane >> 5;
-          const float sum = st.l[0] + __shfl_xor(st.l[0], 32, 64);
+          const float inv = inverse(st.l[0] + __shfl_xor(st.l[0], 32, 64));
           if (row0 + c < rows) {
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             uint16_t* dst = out_row<D>(p, q, kvh, j * BM + row0 + c);
 #pragma unroll
             for (int dt = 0; dt < D / 32; dt++)
 #pragma unroll
-              for (int i = 0; i < 4; i++) {
-                const f32x16_t& o = st.o[0][dt];
-                *reinterpret_cast<u32x2_t*>(dst + 32 * dt + 8 * i + 4 * h) =
-                    u32x2_t{X::pack2(o[4 * i] * inv, o[4 * i + 1] * inv), X::pack2(o[4 * i + 2] * inv, o[4 * i + 3] * inv)};
-              }
+              for (int i = 0; i < 4; i++) store_out<F16>(dst + 32 * dt + 8 * i + 4 * h, st.quad(0, dt, i), inv);
           }
         } else {
-          // through LDS, a wave at a time in its own 64 / 4 KiB, for stores of whole lines
-          float* dst = p.part + slot_of(w, first) * STRIDE;
-          const int lane = tid & 63;
+          // through LDS, 32 dims at a time in the wave's own quarter, for stores of whole lines
+          const int dst = slot_of(w, first) * STRIDE;
+          const int lane = tid & 63, c = lane & 31, h = lane >> 5;
+          float* mine = reinterpret_cast<float*>(lds + wave * (2 * STAGE / WAVES));
 #pragma unroll
           for (int dt = 0; dt < D / 32; dt++) {
-            // [32 rows][32 dims + 4] of one dim block
-            float* mine = reinterpret_cast<float*>(lds + wave * 8192);
-            const int c = lane & 31, h = lane >> 5;
+            wave_lds_sync();
+#pragma unroll
+            for (int i = 0; i < 4; i++) *reinterpret_cast<f32x4_t*>(mine + c * 36 + 8 * i + 4 * h) = st.quad(0, dt, i);
             wave_lds_sync();
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-              const f32x16_t& o = st.o[0][dt];
-              *reinterpret_cast<f32x4_t*>(mine + c * 36 + 8 * i + 4 * h) = f32x4_t{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]};
-            }
-            wave_lds_sync();
-            for (int i = lane; i < 32 * 32; i += 64) {
-              const int row = i >> 5, d = i & 31;
-              if (row0 + row < rows) ap_store(dst + (row0 + row) * D + 32 * dt + d, mine[row * 36 + d]);
+              const int row = 8 * i + (lane >> 3), d = 4 * (lane & 7);
+              if (row0 + row < rows)
+                part.store4(dst + (row0 + row) * D + 32 * dt + d, *reinterpret_cast<const f32x4_t*>(mine + row * 36 + d));
             }
           }
           const float sum = st.l[0] + __shfl_xor(st.l[0], 32, 64);
-          if (lane < 32 && row0 + lane < rows) {
-            ap_store(dst + BM * D + 2 * (row0 + lane), st.m[0]);
-            ap_store(dst + BM * D + 2 * (row0 + lane) + 1, sum);
-          }
+          if (lane < 32 && row0 + lane < rows) part.store2(dst + BM * D + 2 * (row0 + lane), st.m[0], sum);
           merge_if_last<D, F16, BM, THREADS>(p, q, kvh, j, rows, first, last);
         }
         __syncthreads();
@@ -714,7 +732,7 @@ void launch(const PagedArgs& base, int rows, hipStream_t s) {
   if (rows <= 32) {
     a.wgs = NARROW_WGS;
     a.min_units = 8;
-    hipLaunchKernelGGL((attn_paged_narrow_kernel<D, F16, 1, 4, 4>), dim3(a.wgs), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((attn_paged_narrow_kernel<D, F16, 1, 8, 2>), dim3(a.wgs), dim3(512), 0, s, a);
   } else if (rows <= 64) {
     a.wgs = NARROW_WGS;
     a.min_units = 8;

@@ -79,13 +79,6 @@ __device__ __forceinline__ u32x4_t rope8(u32x4_t own, u32x4_t other, u32x4_t c, 
   return r;
 }
 
-// dma16 with the streaming (non-temporal) hint: the cache rows are read once per launch
-__device__ __forceinline__ void dma16_nt(rsrc_t rsrc, uint32_t lds_addr, uint32_t voff, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
-               :
-               : "s"(lds_addr), "v"(voff), "s"(rsrc), "s"(soff));
-}
-
 // device-scope accesses: served at the level all XCDs share
 __device__ __forceinline__ void coherent_store(float* p, float v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);

@@ -131,6 +131,12 @@ __device__ __forceinline__ void dma16(rsrc_t rsrc, uint32_t lds_addr, uint32_t v
                :
                : "s"(lds_addr), "v"(voff), "s"(rsrc), "s"(soff));
 }
+// dma16 with the streaming (non-temporal) hint: for data that is read once per launch
+__device__ __forceinline__ void dma16_nt(rsrc_t rsrc, uint32_t lds_addr, uint32_t voff, uint32_t soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
+               :
+               : "s"(lds_addr), "v"(voff), "s"(rsrc), "s"(soff));
+}
 // The same with the LDS address given as a scalar base plus a compile-time offset: the many destinations of an
 // unrolled loop then cost one live scalar register instead of one each (s_add_u32 leaves its carry in SCC).
 // INST_OFF goes into the instruction's offset field, which moves the LDS address and the memory address alike:
