@@ -36,7 +36,9 @@
 namespace {
 
 constexpr int AP_PAGE_MIN = 16;      // tokens per DMA block
-constexpr int AP_START = 2;          // a tile's start (queries, merge, output) in units
+// a tile's start (first keys under way, queries, merge, output) in units
+constexpr int AP_START_NARROW = 8;
+constexpr int AP_START_WIDE = 2;
 constexpr int AP_MAX_WGS = 1024;     // arrival counters: 4 bytes each at the head of the workspace
 constexpr int64_t AP_COUNTER_BYTES = 4096;
 
@@ -123,6 +125,12 @@ struct Tiles {
   }
 };
 
+// quotient of two numbers of 0 or more, with the short division where they fit
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((uint64_t)(a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
+}
+
 struct Run {                 // a workgroup's run of the sequence, and where it starts
   int64_t x, hi, total;      // cost positions
   int wgs;                   // workgroups that have a run
@@ -130,7 +138,7 @@ struct Run {                 // a workgroup's run of the sequence, and where it 
   int64_t head_cost, off;    // cost of one key head of request r, position inside the request
 };
 
-template <int BM, int TK, int THREADS>
+template <int BM, int TK, int THREADS, int AP_START>
 __device__ __forceinline__ bool find_run(const PagedArgs& p, int w, Run& run) {
   __shared__ int64_t sums[THREADS / 64];
   __shared__ int64_t found[3];
@@ -167,7 +175,7 @@ __device__ __forceinline__ bool find_run(const PagedArgs& p, int w, Run& run) {
   const int64_t most = (total + p.min_units - 1) / p.min_units;
   const int wgs = most < p.wgs ? (int)most : p.wgs;
   if (w >= wgs) return false;                 // the same for the whole workgroup
-  const int64_t lo = total * w / wgs;
+  const int64_t lo = quotient(total * w, wgs);
   if (at <= lo && lo < at + own * p.n_kv) {
     for (int r = r0; r < r1; r++) {
       const int64_t c = cost_of(r);
@@ -182,7 +190,7 @@ __device__ __forceinline__ bool find_run(const PagedArgs& p, int w, Run& run) {
   }
   __syncthreads();
   run.x = lo;
-  run.hi = total * (w + 1) / wgs;
+  run.hi = quotient(total * (w + 1), wgs);
   run.total = total;
   run.wgs = wgs;
   run.r = __builtin_amdgcn_readfirstlane((int)found[0]);
@@ -191,7 +199,7 @@ __device__ __forceinline__ bool find_run(const PagedArgs& p, int w, Run& run) {
   return true;
 }
 // workgroup whose run holds position x: the largest w with floor(total w / wgs) <= x
-__device__ __forceinline__ int wg_of(const Run& run, int64_t x) { return (int)(((x + 1) * run.wgs - 1) / run.total); }
+__device__ __forceinline__ int wg_of(const Run& run, int64_t x) { return (int)quotient((x + 1) * run.wgs - 1, run.total); }
 
 // ---- one wave's share of the products -----------------------------------------------------------------
 // position of a 16-byte chunk in its token's row of the LDS tile
@@ -468,7 +476,7 @@ __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const Pag
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int w = blockIdx.x;
   Run run;
-  if (!find_run<BM, TK, THREADS>(p, w, run)) return;
+  if (!find_run<BM, TK, THREADS, AP_START_NARROW>(p, w, run)) return;
 
   uint32_t voff[block_dmas<D>()];
   block_offsets<D>(voff);
@@ -478,7 +486,7 @@ __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const Pag
   const Partials part(p.part);
 
   int r = run.r;
-  int kvh = (int)(run.off / run.head_cost);
+  int kvh = (int)quotient(run.off, run.head_cost);
   int64_t toff = run.off - kvh * run.head_cost;
   int j = 0;
   bool found = false;
@@ -490,7 +498,7 @@ __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const Pag
     for (; kvh < p.n_kv; kvh++) {
       Tiles<BM, TK> walk(q, p.group);
       for (j = 0; j < tiles; j++) {
-        const int units = walk.next(), cost = units + AP_START;
+        const int units = walk.next(), cost = units + AP_START_NARROW;
         if (!found) {                         // the run's first tile
           if (toff >= cost) {
             toff -= cost;
@@ -501,7 +509,7 @@ __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const Pag
         const int64_t left = run.hi - x;
         if (left <= 0) return;
         const int seg = (int)(toff + left < cost ? toff + left : cost);
-        const int ua = (int)toff > AP_START ? (int)toff - AP_START : 0, ub = seg > AP_START ? seg - AP_START : 0;
+        const int ua = (int)toff > AP_START_NARROW ? (int)toff - AP_START_NARROW : 0, ub = seg > AP_START_NARROW ? seg - AP_START_NARROW : 0;
         const int64_t tile_x = x - toff;
         const int rows = all - j * BM < BM ? all - j * BM : BM;
         const bool begins = toff == 0;
@@ -513,7 +521,8 @@ __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const Pag
           continue;
         }
         if (ua >= ub) continue;
-        const int first = wg_of(run, tile_x + AP_START), last = wg_of(run, tile_x + cost - 1);
+        const int first = tile_x + AP_START_NARROW >= run.x ? w : wg_of(run, tile_x + AP_START_NARROW);
+        const int last = tile_x + cost <= run.hi ? w : wg_of(run, tile_x + cost - 1);
 
         // ---- this wave's units of [ua, ub) ----
         const int n_my = ub - ua > wave ? (ub - ua - wave + WAVES - 1) / WAVES : 0, n_items = 2 * n_my;
@@ -609,7 +618,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs
   // neighbouring runs share keys and values: keep them on one XCD (workgroups go round robin over the eight)
   const int w = (blockIdx.x & 7) * (p.wgs >> 3) + (blockIdx.x >> 3);
   Run run;
-  if (!find_run<BM, TK, THREADS>(p, w, run)) return;
+  if (!find_run<BM, TK, THREADS, AP_START_WIDE>(p, w, run)) return;
 
   uint32_t voff[block_dmas<D>()];
   block_offsets<D>(voff);
@@ -618,7 +627,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs
   const Partials part(p.part);
 
   int r = run.r;
-  int kvh = (int)(run.off / run.head_cost);
+  int kvh = (int)quotient(run.off, run.head_cost);
   int64_t toff = run.off - kvh * run.head_cost;
   bool found = false;
   int64_t x = run.x;
@@ -629,7 +638,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs
     for (; kvh < p.n_kv; kvh++) {
       Tiles<BM, TK> walk(q, p.group);
       for (int j = 0; j < tiles; j++) {
-        const int units = walk.next(), cost = units + AP_START;
+        const int units = walk.next(), cost = units + AP_START_WIDE;
         if (!found) {
           if (toff >= cost) {
             toff -= cost;
@@ -640,7 +649,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs
         const int64_t left = run.hi - x;
         if (left <= 0) return;
         const int seg = (int)(toff + left < cost ? toff + left : cost);
-        const int ua = (int)toff > AP_START ? (int)toff - AP_START : 0, ub = seg > AP_START ? seg - AP_START : 0;
+        const int ua = (int)toff > AP_START_WIDE ? (int)toff - AP_START_WIDE : 0, ub = seg > AP_START_WIDE ? seg - AP_START_WIDE : 0;
         const int64_t tile_x = x - toff;
         const int rows = all - j * BM < BM ? all - j * BM : BM;
         const bool begins = toff == 0;
@@ -652,7 +661,8 @@ __global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs
           continue;
         }
         if (ua >= ub) continue;
-        const int first = wg_of(run, tile_x + AP_START), last = wg_of(run, tile_x + cost - 1);
+        const int first = tile_x + AP_START_WIDE >= run.x ? w : wg_of(run, tile_x + AP_START_WIDE);
+        const int last = tile_x + cost <= run.hi ? w : wg_of(run, tile_x + cost - 1);
 
         const int row0 = 32 * wave;
         const bool active = row0 < rows;
