@@ -203,9 +203,16 @@ __device__ __forceinline__ int wg_of(const Run& run, int64_t x) { return (int)qu
 
 // ---- one wave's share of the products -----------------------------------------------------------------
 // position of a 16-byte chunk in its token's row of the LDS tile
+// (64 banks of 4 bytes: a b128 read serves 16 lanes a cycle - 16 tokens, one chunk -, a transposed b64 read 32 lanes -
+// 4 tokens, 4 chunks.  Both want 16 different chunk places; with 64 dims two tokens share the 256 bytes.)
 template <int D> __device__ __forceinline__ int swz(int t) {
-  if (D == 128) return ((t & 7) << 1) | ((t >> 3) & 1);
-  return (((t >> 1) & 3) << 1) | ((t >> 3) & 1);       // two rows share the 256 bytes of the banks
+  return D == 128 ? ((t & 3) << 2) | ((t >> 2) & 3) : (((t >> 1) & 1) << 2) | ((t >> 2) & 3);
+}
+
+// maximum over a lane and lane ^ 32
+__device__ __forceinline__ float half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // place of element d of a row in the merge area
@@ -232,6 +239,10 @@ struct Wave {
       const uint16_t* src = p.q + ((int64_t)(q.t0 + tok) * p.n_q + kvh * p.group + g) * D + 8 * h;
 #pragma unroll
       for (int s = 0; s < KS; s++) qf[rb][s] = *reinterpret_cast<const bf16x8_t*>(src + 16 * s);
+      // the queries are waited for here, once: left to their first use, the wait would sit in the loop and drain the
+      // DMA in flight at every step
+#pragma unroll
+      for (int s = 0; s < KS; s++) asm volatile("" : "+v"(qf[rb][s]));
       lim[rb] = q.kv - q.n + tok + 1;
       m[rb] = -INFINITY;
       l[rb] = 0.0f;
@@ -243,26 +254,38 @@ struct Wave {
   }
 
   // scores of the unit's keys (LDS tile `ks`, first token tok0), running maximum and sum, probabilities
-  __device__ __forceinline__ void scores(const char* ks, int tok0, bool mask, float c) {
+  template <bool MASK> __device__ __forceinline__ void scores(const char* ks, int tok0, float c) {
     const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
     f32x16_t s[RB][NB];
+    bf16x8_t a[KS][NB];
 #pragma unroll
-    for (int b = 0; b < NB; b++) {
-      const char* base = ks + (32 * b + row) * ROW;
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+        a[k][b] = *reinterpret_cast<const bf16x8_t*>(ks + (32 * b + row) * ROW + (((2 * k + h) ^ swz<D>(row)) << 4));
+#pragma unroll
+    for (int b = 0; b < NB; b++)
 #pragma unroll
       for (int rb = 0; rb < RB; rb++)
 #pragma unroll
         for (int i = 0; i < 16; i++) s[rb][b][i] = 0.0f;
 #pragma unroll
-      for (int k = 0; k < KS; k++) {
-        const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(base + (((2 * k + h) ^ swz<D>(row)) << 4));
+    for (int k = 0; k < KS; k++)
 #pragma unroll
-        for (int rb = 0; rb < RB; rb++) s[rb][b] = X::mfma32(a, qf[rb][k], s[rb][b]);
-      }
+      for (int b = 0; b < NB; b++)        // neighbouring products add to different blocks: none waits for the one before
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) s[rb][b] = X::mfma32(a[k][b], qf[rb][k], s[rb][b]);
+    // fragments are read KS products ahead
+    __builtin_amdgcn_sched_group_barrier(SG_DS_RD, KS, 0);
+#pragma unroll
+    for (int i = 0; i < (NB - 1) * KS; i++) {
+      __builtin_amdgcn_sched_group_barrier(SG_MFMA, RB, 0);
+      __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 1, 0);
     }
+    __builtin_amdgcn_sched_group_barrier(SG_MFMA, KS * RB, 0);
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) {
-      if (mask) {
+      if (MASK) {
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -274,7 +297,7 @@ struct Wave {
       for (int b = 0; b < NB; b++)
 #pragma unroll
         for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[rb][b][i]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      mx = half_max(mx);
       // The maximum only has to keep the exponentials in range: it is moved (and O and l rescaled) when a row's has
       // grown by more than 8 binary orders, not at every step.  A row that has seen nothing yet stays at -inf.
       if (__any((mx - m[rb]) * c > 8.0f)) {
@@ -288,20 +311,19 @@ struct Wave {
           for (int i = 0; i < 16; i++) o[rb][dt][i] *= f;
       }
       const float mc = m[rb] == -INFINITY ? 0.0f : m[rb] * c;
-      float sum = 0.0f;
+      // the sum takes the probabilities as the second product sees them, rounded: half as many instructions (a dot
+      // product with ones adds two), and numerator and denominator then share each rounding
 #pragma unroll
       for (int b = 0; b < NB; b++) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          s[rb][b][i] = __builtin_amdgcn_exp2f(fmaf(s[rb][b][i], c, -mc));
-          sum += s[rb][b][i];
-        }
+        for (int i = 0; i < 16; i++) s[rb][b][i] = __builtin_amdgcn_exp2f(fmaf(s[rb][b][i], c, -mc));
 #pragma unroll
-        for (int k = 0; k < 2; k++)
+        for (int k = 0; k < 2; k++) {
 #pragma unroll
           for (int e = 0; e < 4; e++) pf[rb][2 * b + k][e] = X::pack2(s[rb][b][8 * k + 2 * e], s[rb][b][8 * k + 2 * e + 1]);
+          l[rb] = X::sum8(__builtin_bit_cast(bf16x8_t, pf[rb][2 * b + k]), l[rb]);
+        }
       }
-      l[rb] += sum;
     }
   }
 
@@ -309,20 +331,33 @@ struct Wave {
   __device__ __forceinline__ void values(const char* vs) {
     const int lane = threadIdx.x & 63, i16 = lane & 15, half = (lane >> 4) & 1, h = lane >> 5;
     const int t = 4 * h + (i16 >> 2);
+    auto fragment = [&](int k, int dt) {
+      const int chunk = 4 * dt + 2 * half + ((i16 & 3) >> 1);
+      const char* a = vs + (16 * k + t) * ROW + ((chunk ^ swz<D>(t)) << 4) + 8 * (i16 & 1);
+      const char* b = vs + (16 * k + t + 8) * ROW + ((chunk ^ swz<D>(t + 8)) << 4) + 8 * (i16 & 1);
+      const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((bf16x4_t __attribute__((address_space(3)))*)(a));
+      const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((bf16x4_t __attribute__((address_space(3)))*)(b));
+      return (bf16x8_t)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    bf16x8_t vf[2 * NB][DT];
 #pragma unroll
-    for (int k = 0; k < 2 * NB; k++) {
+    for (int k = 0; k < 2 * NB; k++)
 #pragma unroll
-      for (int dt = 0; dt < DT; dt++) {
-        const int chunk = 4 * dt + 2 * half + ((i16 & 3) >> 1);
-        const char* a = vs + (16 * k + t) * ROW + ((chunk ^ swz<D>(t)) << 4) + 8 * (i16 & 1);
-        const char* b = vs + (16 * k + t + 8) * ROW + ((chunk ^ swz<D>(t + 8)) << 4) + 8 * (i16 & 1);
-        const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((bf16x4_t __attribute__((address_space(3)))*)(a));
-        const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((bf16x4_t __attribute__((address_space(3)))*)(b));
-        const bf16x8_t vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      for (int dt = 0; dt < DT; dt++) vf[k][dt] = fragment(k, dt);
 #pragma unroll
-        for (int rb = 0; rb < RB; rb++) o[rb][dt] = X::mfma32(vf, __builtin_bit_cast(bf16x8_t, pf[rb][k]), o[rb][dt]);
-      }
+    for (int k = 0; k < 2 * NB; k++)
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) o[rb][dt] = X::mfma32(vf[k][dt], __builtin_bit_cast(bf16x8_t, pf[rb][k]), o[rb][dt]);
+    // 16 tokens' fragments are read while the previous ones' are multiplied
+    __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 2 * DT, 1);
+#pragma unroll
+    for (int i = 0; i < (2 * NB - 1) * DT; i++) {
+      __builtin_amdgcn_sched_group_barrier(SG_MFMA, RB, 1);
+      __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 2, 1);
     }
+    __builtin_amdgcn_sched_group_barrier(SG_MFMA, DT * RB, 1);
   }
 
   // four consecutive dims of the lane's row: 32 dt + 8 i + 4 h
@@ -526,6 +561,8 @@ __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const Pag
 
         // ---- this wave's units of [ua, ub) ----
         const int n_my = ub - ua > wave ? (ub - ua - wave + WAVES - 1) / WAVES : 0, n_items = 2 * n_my;
+        Wave<D, F16, RB, 1> st;
+        st.start(p, q, kvh, j * BM, all);
         int pg[2];
         auto fetch_pages = [&](int i) {
           const int tok = (ua + wave + WAVES * i) * TK;
@@ -556,14 +593,13 @@ __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const Pag
 #pragma unroll
         for (int it = 0; it < AHEAD; it++)
           if (it < n_items) issue(it);
-        Wave<D, F16, RB, 1> st;
-        st.start(p, q, kvh, j * BM, all);
-        const int lim0 = q.kv - q.n + (j * BM) / p.group + 1;   // what the tile's first row sees
         for (int i = 0; i < n_my; i++) {
           const int tok = (ua + wave + WAVES * i) * TK;
           if (2 * i + AHEAD < n_items) issue(2 * i + AHEAD);
           wait_item(2 * i);
-          st.scores(ring + ((2 * i) % RING) * ITEM, tok, tok + TK > lim0, p.scale_log2e);
+          // always with the mask: it hides behind the memory, and a second path without it made the compiler copy the
+          // accumulators where the two meet (decode of 64 requests 98 -> 114 us)
+          st.template scores<true>(ring + ((2 * i) % RING) * ITEM, tok, p.scale_log2e);
           if (2 * i + 1 + AHEAD < n_items) issue(2 * i + 1 + AHEAD);
           wait_item(2 * i + 1);
           st.values(ring + ((2 * i + 1) % RING) * ITEM);
@@ -668,9 +704,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs
         const bool active = row0 < rows;
         Wave<D, F16, 1, 2> st;
         st.start(p, q, kvh, j * BM + row0, all);
-        // tokens seen by the wave's first and last row
-        const int last_row = j * BM + (row0 + 31 < rows ? row0 + 31 : rows - 1);
-        const int lim0 = q.kv - q.n + (j * BM + row0) / p.group + 1, lim1 = q.kv - q.n + last_row / p.group + 1;
+        const int lim0 = q.kv - q.n + (j * BM + row0) / p.group + 1;   // what the wave's first row sees
         int page = page_at(p, r, q.kv, ua * TK + wave * AP_PAGE_MIN);
         auto issue = [&](int u) {
           const int tok = u * TK + wave * AP_PAGE_MIN;
@@ -682,15 +716,29 @@ __global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs
           if (u + 1 < ub) page = page_at(p, r, q.kv, tok + TK);
         };
         issue(ua);
-        for (int u = ua; u < ub; u++) {
+        auto step = [&](int u) {              // unit u has arrived, unit u - 1 has been read by all
           wait_vm_at_most<0>();
-          __syncthreads();                    // unit u has arrived, unit u - 1 has been read by all
+          __syncthreads();
           if (u + 1 < ub) issue(u + 1);
-          if (active && u * TK < lim1) {
+        };
+        if (active) {
+          int free_of_mask = lim0 <= 0 ? 0 : lim0 / TK;      // units that all of the wave's rows see whole
+          if (free_of_mask > ub) free_of_mask = ub;
+          int u = ua;
+          for (; u < free_of_mask; u++) {
+            step(u);
             const char* base = lds + (u & 1) * STAGE;
-            st.scores(base, u * TK, u * TK + TK > lim0, p.scale_log2e);
+            st.template scores<false>(base, u * TK, p.scale_log2e);
             st.values(base + HALF);
           }
+          for (; u < ub; u++) {
+            step(u);
+            const char* base = lds + (u & 1) * STAGE;
+            st.template scores<true>(base, u * TK, p.scale_log2e);
+            st.values(base + HALF);
+          }
+        } else {                              // no such rows: the wave brings keys and values for the others
+          for (int u = ua; u < ub; u++) step(u);
         }
         __syncthreads();
 

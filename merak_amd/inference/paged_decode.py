@@ -1,0 +1,146 @@
+"""Llama-shaped models served over a paged key/value cache: prompts in chunks, single tokens and drafted tokens of many
+requests in one step.
+
+The reference's generation loop pushes the whole token buffer of one batch through the model for every new token
+(Merak/inference/text_generation_inference.py:199-203).  ``LlamaDecoder`` keeps one cache row per sequence and takes one
+token at a time; here requests come and go, bring any number of tokens each, and share a pool of pages.
+
+A step of ``PagedLlamaDecoder``: ``ops.paged_plan`` hands out pages, positions and slots from the lengths, and per block
+the QKV product, ``ops.qk_norm_rope_append`` (rotary embedding, optional norms of the query and key heads, keys and
+values to their pages), ``ops.attn_paged``, and the block's other products.  Everything that depends on lengths lives on
+the device.  ``verify`` runs the drafts of every request through one such step and keeps what ``ops.verify_draft``
+accepts.
+"""
+from __future__ import annotations
+
+from typing import List, Optional, Sequence, Tuple
+
+import torch
+
+from .. import ops
+from .llama_decode import LlamaBlockWeights, LlamaDecoder, rope_tables
+
+
+class PagedLlamaDecoder:
+    """``slots`` requests over ``n_pages`` pages of ``page_size`` tokens per layer.
+
+    ``append(tokens, new_lens)`` adds ``new_lens[r]`` tokens to request r (host numbers; the tokens of all requests one
+    after the other) and returns the final-norm output of every new token.  A request that finds no page is refused:
+    ``self.granted[r]`` is False, its rows are meaningless and its state is as before.  ``release(r)`` gives a request's
+    pages back.  ``q_norms`` / ``k_norms``: norm weights [head_dim] of each block's query and key heads, for models that
+    have them."""
+
+    def __init__(self, embed: torch.Tensor, blocks: List[LlamaBlockWeights], final_norm: torch.Tensor,
+                 lm_head: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim: int = 128, eps: float = 1e-5,
+                 rope_theta: float = 10000.0, rope_scaling: Optional[dict] = None, max_len: int = 4096, slots: int = 8,
+                 page_size: int = 64, n_pages: Optional[int] = None, q_norms: Optional[Sequence[torch.Tensor]] = None,
+                 k_norms: Optional[Sequence[torch.Tensor]] = None):
+        dev, dt = lm_head.device, lm_head.dtype
+        self.embed, self.blocks, self.final_norm, self.lm_head = embed, blocks, final_norm, lm_head
+        self.n_q, self.n_kv, self.head_dim, self.eps = n_q_heads, n_kv_heads, head_dim, eps
+        self.max_len, self.slots, self.page_size = max_len, slots, page_size
+        self.q_norms = list(q_norms) if q_norms is not None else [None] * len(blocks)
+        self.k_norms = list(k_norms) if k_norms is not None else [None] * len(blocks)
+        if len(self.q_norms) != len(blocks) or len(self.k_norms) != len(blocks):
+            raise ValueError("q_norms and k_norms need one entry per block")
+        per_request = -(-max_len // page_size)
+        n_pages = slots * per_request if n_pages is None else n_pages
+        cache = lambda: torch.zeros((n_pages, n_kv_heads, page_size, head_dim), dtype=dt, device=dev)
+        self.k_cache = [cache() for _ in blocks]
+        self.v_cache = [cache() for _ in blocks]
+        self.cos, self.sin = rope_tables(head_dim, max_len, rope_theta, rope_scaling, dtype=torch.float32, device=dev)
+        self.lens = torch.zeros((slots,), dtype=torch.int64, device=dev)
+        self.held = torch.zeros((slots,), dtype=torch.int32, device=dev)
+        self.block_tables = torch.full((slots, per_request), -1, dtype=torch.int32, device=dev)
+        self.free_pages = torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=dev)
+        self.free_count = torch.tensor([n_pages], dtype=torch.int32, device=dev)
+        self.granted = torch.ones((slots,), dtype=torch.bool, device=dev)
+        self.attn_ws = ops.attn_paged_workspace(dev)
+        self._dev = dev
+
+    @classmethod
+    def from_hf(cls, model, **kw):
+        """From a ``transformers`` Llama-shaped causal model (weights as ``LlamaDecoder.from_hf`` lays them out); norms of
+        the query and key heads are taken where its attention has ``q_norm`` / ``k_norm``."""
+        base = LlamaDecoder.from_hf(model, max_len=1, batch=1)
+        cfg = model.config
+        rp = getattr(cfg, "rope_parameters", None) or getattr(cfg, "rope_scaling", None) or {}
+        layers = [layer.self_attn for layer in model.model.layers]
+        if hasattr(layers[0], "q_norm"):
+            kw.setdefault("q_norms", [a.q_norm.weight.data for a in layers])
+            kw.setdefault("k_norms", [a.k_norm.weight.data for a in layers])
+        return cls(base.embed, base.blocks, base.final_norm, base.lm_head, base.n_q, base.n_kv, base.head_dim, base.eps,
+                   rp.get("rope_theta", getattr(cfg, "rope_theta", 10000.0)),
+                   rp if rp.get("rope_type", "default") != "default" else None, **kw)
+
+    def release(self, finished: Sequence[int]) -> None:
+        """The pages of these requests go back to the pool; their lengths become 0."""
+        mask = torch.zeros((self.slots,), dtype=torch.bool)
+        mask[list(finished)] = True
+        mask = mask.to(self._dev)
+        ops.paged_release(mask, self.held, self.block_tables, self.free_pages, self.free_count)
+        self.lens.masked_fill_(mask, 0)
+
+    def append(self, tokens: torch.Tensor, new_lens: Sequence[int]) -> torch.Tensor:
+        """``tokens`` int64 [sum(new_lens)] -> hidden [sum(new_lens), H] after the final norm."""
+        new_lens = [int(n) for n in new_lens]
+        T = sum(new_lens)
+        if len(new_lens) != self.slots or min(new_lens) < 0 or tokens.shape != (T,):
+            raise ValueError(f"append: {tuple(tokens.shape)} tokens for new_lens {new_lens} of {self.slots} requests")
+        new = torch.tensor(new_lens, dtype=torch.int64).to(self._dev)
+        plan = ops.paged_plan(self.lens, new, self.held, self.block_tables, self.free_pages, self.free_count,
+                              self.page_size, T)
+        self.held, self.free_count, self.granted = plan.held, plan.free_count, plan.granted
+        self.lens = torch.where(plan.granted, self.lens + new, self.lens)
+        x = ops.embedding_gather(tokens, self.embed, 0, self.embed.shape[0])
+        if T == 0:
+            return x
+        residual, most = None, max(new_lens)
+        for i, w in enumerate(self.blocks):
+            h, residual = ops.rmsnorm(x, w.input_norm, self.eps, residual, want_residual=True)
+            qkv = ops.linear_fwd(h, w.qkv, None)[0]
+            q = ops.qk_norm_rope_append(qkv, self.cos, self.sin, plan.positions, plan.slots, self.k_cache[i],
+                                        self.v_cache[i], self.n_q, self.q_norms[i], self.k_norms[i], self.eps)
+            a = ops.attn_paged(q, self.k_cache[i], self.v_cache[i], self.block_tables, plan.cu, plan.kv_lens, max_new=most,
+                               workspace=self.attn_ws)
+            o = ops.linear_fwd(a.view(T, -1), w.o, None)[0]
+            h, residual = ops.rmsnorm(o, w.post_norm, self.eps, residual, want_residual=True)
+            act = ops.linear_fwd(h, w.gate_up, None, ops.EPI_SWIGLU, want_pre=False)[1]
+            x = ops.linear_fwd(act, w.down, None)[0]
+        return ops.rmsnorm(x, self.final_norm, self.eps, residual)
+
+    def logits(self, hidden: torch.Tensor) -> torch.Tensor:
+        return ops.linear_fwd(hidden, self.lm_head, None)[0]
+
+    def step(self, tokens: torch.Tensor, new_lens: Sequence[int]) -> torch.Tensor:
+        """Greedy next token of every request that brought tokens (int64 [slots], -1 for the others): what the reference
+        picks at :223-227 from the last position."""
+        hidden = self.append(tokens, new_lens)
+        last = torch.tensor(new_lens).cumsum(0) - 1
+        who = [r for r, n in enumerate(new_lens) if n]
+        out = torch.full((self.slots,), -1, dtype=torch.int64, device=self._dev)
+        if who:
+            rows = hidden[last[who].to(self._dev)]
+            out[torch.tensor(who).to(self._dev)] = ops.argmax_rows(self.logits(rows))
+        return out
+
+    def verify(self, last_tokens: torch.Tensor, draft_tokens: torch.Tensor, uniforms: torch.Tensor,
+               draft_probs: Optional[torch.Tensor] = None, temperature: float = 1.0, top_k: int = 0, top_p: float = 0.0
+               ) -> Tuple[torch.Tensor, torch.Tensor]:
+        """One step of speculative decoding for all requests: ``last_tokens`` int64 [slots] (not yet in the cache) and
+        ``draft_tokens`` int64 [slots, K] go through the model together, the sampling tail's filter and softmax give the
+        target's probabilities, and ``ops.verify_draft`` decides.  -> (tokens [slots, K + 1], accepted [slots]); the
+        cache keeps ``last_tokens`` and the accepted drafts, the last of ``tokens`` is the next call's ``last_tokens``.
+        ``draft_probs`` fp32 [slots, K, V], or None for drafts without probabilities of their own; ``uniforms`` fp32
+        [slots, K + 1]."""
+        R, K = draft_tokens.shape
+        if R != self.slots or last_tokens.shape != (R,):
+            raise ValueError(f"verify: {tuple(last_tokens.shape)} tokens and {tuple(draft_tokens.shape)} drafts for "
+                             f"{self.slots} requests")
+        before = self.lens
+        hidden = self.append(torch.cat([last_tokens[:, None], draft_tokens], 1).reshape(-1), [K + 1] * R)
+        z = ops.sample_top_k_top_p(self.logits(hidden), temperature, top_k, top_p, None, want_filtered=True)[1]
+        tokens, accepted = ops.verify_draft(draft_tokens, torch.softmax(z, -1).view(R, K + 1, -1), draft_probs, uniforms)
+        # rejected drafts leave the cache by the length alone: their slots are written again by the next tokens
+        self.lens = torch.where(self.granted, before + 1 + accepted, before)
+        return tokens, accepted

@@ -51,7 +51,25 @@ def _require_gpu(*ts: torch.Tensor) -> torch.device:
 
 
 def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(dev.index)   # without the Stream object around it: 1.8 us of a small launch
+
+
+class _Here:
+    """Stands in for ``torch.cuda.device(dev)`` where dev is the current device already: entering and leaving that
+    takes as long as a small launch."""
+
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _device(dev: torch.device):
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _p(t: Optional[torch.Tensor]):
@@ -708,7 +726,7 @@ class PagedPlan(NamedTuple):
 
 
 def _index(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape: Tuple[int, ...]) -> torch.Tensor:
-    if t.dtype != dtype or tuple(t.shape) != shape:
+    if t.dtype is not dtype or t.shape != shape:
         raise ValueError(f"{what}: {name} must be {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
     return _contig(t)
 
@@ -749,10 +767,12 @@ def paged_plan(lens: torch.Tensor, new_lens: torch.Tensor, held: torch.Tensor, b
     tokens = int(tokens)
     if tokens < 0:
         raise ValueError(f"paged_plan: tokens={tokens}")
-    i64 = lambda n: torch.empty((n,), dtype=torch.int64, device=dev)
-    plan = PagedPlan(i64(tokens), i64(tokens), i64(R + 1), i64(R), torch.empty((R,), dtype=torch.bool, device=dev),
-                     torch.empty_like(held), torch.empty_like(free_count))
-    with torch.cuda.device(dev):
+    # two allocations for seven small results: the allocator costs more than the kernel
+    wide = torch.empty((2 * tokens + 2 * R + 1,), dtype=torch.int64, device=dev)
+    narrow = torch.empty((2 * R + 1,), dtype=torch.int32, device=dev)
+    new_held, count, flags = narrow.split((R, 1, R))
+    plan = PagedPlan(*wide.split((tokens, tokens, R + 1, R)), flags.view(torch.bool)[:R], new_held, count)
+    with _device(dev):
         _lib.check(_lib.lib().mtp_paged_plan(_p(lens), _p(new_lens), _p(held), _p(block_tables), _p(free_pages),
                                              _p(free_count), _p(plan.slots), _p(plan.positions), _p(plan.cu),
                                              _p(plan.kv_lens), _p(plan.granted), _p(plan.held), _p(plan.free_count), R,
@@ -772,7 +792,7 @@ def paged_release(finished: torch.Tensor, held: torch.Tensor, block_tables: torc
     finished = _index("paged_release", "finished", finished, torch.bool, (R,))
     for name, t, n in (("held", held, R), ("free_pages", free_pages, free_pages.numel()), ("free_count", free_count, 1)):
         _index("paged_release", name, _own("paged_release", name, t), torch.int32, (n,))
-    with torch.cuda.device(dev):
+    with _device(dev):
         _lib.check(_lib.lib().mtp_paged_release(_p(finished), _p(held), _p(_contig(block_tables)), _p(free_pages),
                                                 _p(free_count), R, max_pages, free_pages.numel(), _stream(dev)),
                    "mtp_paged_release")
@@ -818,7 +838,7 @@ def qk_norm_rope(qkv: torch.Tensor, cos_table: torch.Tensor, sin_table: torch.Te
                                                            n_kv, q_weight, k_weight)
     q = torch.empty((T, n_q_heads, hd), dtype=qkv.dtype, device=dev)
     k = torch.empty((T, n_kv, hd), dtype=qkv.dtype, device=dev)
-    with torch.cuda.device(dev):
+    with _device(dev):
         _lib.check(_lib.lib().mtp_qk_norm_rope(_p(qkv), _p(cos), _p(sin), _dt(cos), _p(positions), _p(qw), _p(kw), _p(q),
                                                _p(k), T, n_q_heads, n_kv, hd, cos.shape[0], float(eps), _dt(qkv),
                                                _stream(dev)), "mtp_qk_norm_rope")
@@ -853,7 +873,7 @@ def qk_norm_rope_bwd(dq: Optional[torch.Tensor], dk: Optional[torch.Tensor], dv:
     if dqw is not None or dkw is not None:
         need = lib.mtp_qk_norm_rope_bwd_workspace_bytes(T, n_q_heads, n_kv, hd)
         ws = torch.empty((max(int(need), 4),), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
+    with _device(dev):
         _lib.check(lib.mtp_qk_norm_rope_bwd(_p(dq), _p(dk), _p(dv), _p(qkv), _p(cos), _p(sin), _dt(cos), _p(positions),
                                             _p(qw), _p(kw), _p(dqkv), _p(dqw), _p(dkw), _p(ws),
                                             0 if ws is None else ws.numel(), T, n_q_heads, n_kv, hd, cos.shape[0],
@@ -881,7 +901,7 @@ def qk_norm_rope_append(qkv: torch.Tensor, cos_table: torch.Tensor, sin_table: t
                                                            n_q_heads, n_kv, q_weight, k_weight)
     slots = _index("qk_norm_rope_append", "slots", slots, torch.int64, (T,))
     q = torch.empty((T, n_q_heads, hd), dtype=qkv.dtype, device=dev)
-    with torch.cuda.device(dev):
+    with _device(dev):
         _lib.check(_lib.lib().mtp_qk_norm_rope_append(_p(qkv), _p(cos), _p(sin), _dt(cos), _p(positions), _p(slots), _p(qw),
                                                       _p(kw), _p(q), _p(k_cache), _p(v_cache), T, n_q_heads, n_kv, hd,
                                                       cos.shape[0], n_pages, page_size, float(eps), _dt(qkv),
@@ -928,7 +948,7 @@ def attn_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
         raise ValueError("attn_paged: out must be a contiguous, 16-byte aligned tensor like q")
     if workspace is None:
         workspace = attn_paged_workspace(dev)
-    with torch.cuda.device(dev):
+    with _device(dev):
         _lib.check(_lib.lib().mtp_attn_paged(_p(q), _p(k_cache), _p(v_cache), _p(block_tables), _p(cu), _p(kv_lens), _p(out),
                                              _p(workspace), workspace.numel() * workspace.element_size(), T, R, n_q, n_kv,
                                              hd, n_pages, page_size, max_pages, max_new, len_bound, scale, _dt(q),
@@ -962,7 +982,7 @@ def verify_draft(draft_tokens: torch.Tensor, target_probs: torch.Tensor, draft_p
     lib = _lib.lib()
     need = int(lib.mtp_verify_draft_workspace_bytes(R, V))
     ws = torch.empty((max(need, 8),), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
+    with _device(dev):
         _lib.check(lib.mtp_verify_draft(_p(draft_tokens), _p(draft_lens), _p(target_probs), _p(draft_probs), _p(uniforms),
                                         _p(tokens), _p(accepted), _p(ws), ws.numel(), R, K, V, _dt(target_probs),
                                         _stream(dev)), "mtp_verify_draft")
