@@ -30,7 +30,7 @@
 // Two kernels, chosen by the most rows a tile can have:
 //   narrow  up to 32 RB rows (RB = 1, 2), bound by HBM: the waves of a workgroup take turns with the units of its run,
 //           each with a ring of LDS slots of its own and no barrier in the loop, and are merged at the end;
-//   wide    128 rows, 32 per wave, bound by the matrix cores: the waves share each unit's keys and values.
+//   wide    256 rows, 32 per wave, bound by the matrix cores: the waves share each unit's keys and values.
 #include "gemm_bf16_kernel.h"
 
 namespace {
@@ -38,7 +38,7 @@ namespace {
 constexpr int AP_PAGE_MIN = 16;      // tokens per DMA block
 // a tile's start (first keys under way, queries, merge, output) in units
 constexpr int AP_START_NARROW = 8;
-constexpr int AP_START_WIDE = 2;
+constexpr int AP_START_WIDE = 4;
 constexpr int AP_MAX_WGS = 1024;     // arrival counters: 4 bytes each at the head of the workspace
 constexpr int64_t AP_COUNTER_BYTES = 4096;
 
@@ -644,11 +644,11 @@ __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const Pag
 
 // ---- wide tiles: the waves share the units --------------------------------------------------------------
 template <int D, bool F16>
-__global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs p) {
-  constexpr int TK = 64, WAVES = 4, BM = 32 * WAVES, THREADS = 256;
+__global__ __launch_bounds__(512, 2) void attn_paged_wide_kernel(const PagedArgs p) {
+  constexpr int WAVES = 8, STAGES = 4, TK = 64, BM = 32 * WAVES, THREADS = WAVES * 64;
   constexpr int HALF = TK * D * 2, STAGE = 2 * HALF;     // keys, then values of one unit
-  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
-  __shared__ float ml[WAVES][64];
+  constexpr int DMAS = block_dmas<D>();                  // of the unit's 8 blocks (4 of keys, 4 of values) a wave brings one
+  __shared__ __attribute__((aligned(1024))) char lds[STAGES * STAGE];
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // neighbouring runs share keys and values: keep them on one XCD (workgroups go round robin over the eight)
@@ -658,7 +658,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs
 
   uint32_t voff[block_dmas<D>()];
   block_offsets<D>(voff);
-  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr_of(lds)) + wave * (AP_PAGE_MIN * D * 2);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr_of(lds)) + (wave & 3) * (AP_PAGE_MIN * D * 2);
   constexpr int STRIDE = BM * (D + 2);
   const Partials part(p.part);
 
@@ -705,35 +705,41 @@ __global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs
         Wave<D, F16, 1, 2> st;
         st.start(p, q, kvh, j * BM + row0, all);
         const int lim0 = q.kv - q.n + (j * BM + row0) / p.group + 1;   // what the wave's first row sees
-        int page = page_at(p, r, q.kv, ua * TK + wave * AP_PAGE_MIN);
+        int page = page_at(p, r, q.kv, ua * TK + (wave & 3) * AP_PAGE_MIN);
         auto issue = [&](int u) {
-          const int tok = u * TK + wave * AP_PAGE_MIN;
+          const int tok = u * TK + (wave & 3) * AP_PAGE_MIN;
           int tokens;
           const int64_t at = block_at<D>(p, page, kvh, q.kv, tok, tokens);
-          const uint32_t dst = lds0 + (u & 1) * STAGE;
-          dma_block<D, false>(p.k, at, tokens, dst, voff);
-          dma_block<D, false>(p.v, at, tokens, dst + HALF, voff);
+          const uint32_t dst = lds0 + (uint32_t)(u % STAGES) * STAGE;
+          if (wave < 4) dma_block<D, false>(p.k, at, tokens, dst, voff);
+          else dma_block<D, false>(p.v, at, tokens, dst + HALF, voff);
           if (u + 1 < ub) page = page_at(p, r, q.kv, tok + TK);
         };
-        issue(ua);
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; i++)
+          if (ua + i < ub) issue(ua + i);
         auto step = [&](int u) {              // unit u has arrived, unit u - 1 has been read by all
-          wait_vm_at_most<0>();
+          const int after = ub - 1 - u;       // units requested behind u: up to STAGES - 2
+          if (after >= STAGES - 2) wait_vm_at_most<(STAGES - 2) * DMAS>();
+          else if (after == 1) wait_vm_at_most<DMAS>();
+          else wait_vm_at_most<0>();
           __syncthreads();
-          if (u + 1 < ub) issue(u + 1);
+          if (u + STAGES - 1 < ub) issue(u + STAGES - 1);
         };
+        static_assert(STAGES == 4, "step");
         if (active) {
           int free_of_mask = lim0 <= 0 ? 0 : lim0 / TK;      // units that all of the wave's rows see whole
           if (free_of_mask > ub) free_of_mask = ub;
           int u = ua;
           for (; u < free_of_mask; u++) {
             step(u);
-            const char* base = lds + (u & 1) * STAGE;
+            const char* base = lds + (u % STAGES) * STAGE;
             st.template scores<false>(base, u * TK, p.scale_log2e);
             st.values(base + HALF);
           }
           for (; u < ub; u++) {
             step(u);
-            const char* base = lds + (u & 1) * STAGE;
+            const char* base = lds + (u % STAGES) * STAGE;
             st.template scores<true>(base, u * TK, p.scale_log2e);
             st.values(base + HALF);
           }
@@ -756,7 +762,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs
           // through LDS, 32 dims at a time in the wave's own quarter, for stores of whole lines
           const int dst = slot_of(w, first) * STRIDE;
           const int lane = tid & 63, c = lane & 31, h = lane >> 5;
-          float* mine = reinterpret_cast<float*>(lds + wave * (2 * STAGE / WAVES));
+          float* mine = reinterpret_cast<float*>(lds + wave * (STAGES * STAGE / WAVES));
 #pragma unroll
           for (int dt = 0; dt < D / 32; dt++) {
             wave_lds_sync();
@@ -782,7 +788,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_wide_kernel(const PagedArgs
 }
 
 constexpr int NARROW_WGS = 256;      // one per CU: 128 KiB of LDS each
-constexpr int WIDE_WGS = 512;        // two per CU: 64 KiB each
+constexpr int WIDE_WGS = 256;        // one per CU: 128 KiB
 
 template <int D, bool F16>
 void launch(const PagedArgs& base, int rows, hipStream_t s) {
@@ -798,14 +804,14 @@ void launch(const PagedArgs& base, int rows, hipStream_t s) {
   } else {
     a.wgs = WIDE_WGS;
     a.min_units = 4;
-    hipLaunchKernelGGL((attn_paged_wide_kernel<D, F16>), dim3(a.wgs), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((attn_paged_wide_kernel<D, F16>), dim3(a.wgs), dim3(512), 0, s, a);
   }
 }
 
 }  // namespace
 
 extern "C" int64_t mtp_attn_paged_workspace_bytes(void) {
-  return AP_COUNTER_BYTES + 2ll * WIDE_WGS * 128 * (128 + 2) * (int64_t)sizeof(float);
+  return AP_COUNTER_BYTES + 2ll * WIDE_WGS * 256 * (128 + 2) * (int64_t)sizeof(float);
 }
 
 extern "C" int mtp_attn_paged(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables,

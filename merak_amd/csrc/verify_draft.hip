@@ -79,10 +79,31 @@ struct Row {
     q = rejected && a.draft ? static_cast<const T*>(a.draft) + (r * a.K + n) * a.V : nullptr;
     without = rejected && !a.draft ? a.drafts[r * a.K + n] : -1;
   }
-  __device__ __forceinline__ void at(int64_t v, double& left, double& whole) const {
-    const double pv = (double)to_f32(p[v]);
-    whole = weight_of(pv);
-    left = q ? weight_of(pv - (double)to_f32(q[v])) : v == without ? 0.0 : whole;
+  // weights of the 8 elements at, at + step, ... below end (0 behind it): left over and whole.  All loads are issued
+  // together, from clamped places: a branch around each would wait for each.
+  __device__ __forceinline__ void load8(int64_t at, int step, int64_t end, double* left, double* whole) const {
+    float pv[8], qv[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int64_t v = at + j * step < end ? at + j * step : end - 1;
+      pv[j] = to_f32(p[v]);
+    }
+    if (q) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int64_t v = at + j * step < end ? at + j * step : end - 1;
+        qv[j] = to_f32(q[v]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) qv[j] = at + j * step == without ? INFINITY : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const bool in = at + j * step < end;
+      whole[j] = in ? weight_of((double)pv[j]) : 0.0;
+      left[j] = in ? weight_of((double)pv[j] - (double)qv[j]) : 0.0;
+    }
   }
 };
 
@@ -103,12 +124,7 @@ __global__ __launch_bounds__(VD_THREADS) void verify_sum_kernel(const VerifyArgs
   double left = 0.0, whole = 0.0;
   for (int64_t v = v0 + threadIdx.x; v < v1; v += VD_STEP) {
     double l[8], w[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const int64_t at = v + j * VD_THREADS;
-      l[j] = w[j] = 0.0;
-      if (at < v1) row.at(at, l[j], w[j]);
-    }
+    row.load8(v, VD_THREADS, v1, l, w);
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       left += l[j];
@@ -172,45 +188,55 @@ __global__ __launch_bounds__(VD_THREADS) void verify_draw_kernel(const VerifyArg
   }
   __syncthreads();
   if (chunk >= 0) {
-    // consecutive elements per thread, twice: their sum, then the walk to the border
+    // 2048 elements at a time, 8 consecutive ones per thread, loaded together and kept: their sum, then the walk to the
+    // border in the thread whose range holds it
     const int64_t v0 = (int64_t)chunk * p.chunk_len;
     const int64_t v1 = v0 + p.chunk_len < p.V ? v0 + p.chunk_len : p.V;
-    const int per = p.chunk_len / VD_THREADS;
-    const int64_t a = v0 + (int64_t)tid * per;
-    double own = 0.0;
-    int64_t last_mine = -1;
-    for (int j = 0; j < per; j++)
-      if (a + j < v1) {
-        double l, w;
-        row.at(a + j, l, w);
-        const double x = use_left ? l : w;
-        own += x;
-        if (x > 0.0) last_mine = a + j;
-      }
-    const double scan = wave_scan_f64(own);
-    if (lane == 63) sums[wave] = scan;
-    __syncthreads();
     double base = before;
+    int64_t last_mine = -1;
+    for (int64_t s0 = v0; s0 < v1; s0 += VD_STEP) {
+      const int64_t a = s0 + 8 * tid;
+      double l[8], x[8], own = 0.0;
+      row.load8(a, 1, v1, l, x);
 #pragma unroll
-    for (int w = 0; w < VD_WAVES; w++)
-      if (w < wave) base += sums[w];
-    double run = base + (scan - own);
-    int64_t here = p.V;
-    if (own > 0.0 && base + scan > point) {
-      for (int j = 0; j < per && here == p.V; j++)
-        if (a + j < v1) {
-          double l, w;
-          row.at(a + j, l, w);
-          const double x = use_left ? l : w;
-          run += x;
-          if (x > 0.0 && run > point) here = a + j;
+      for (int j = 0; j < 8; j++) {
+        x[j] = use_left ? l[j] : x[j];
+        own += x[j];
+        if (x[j] > 0.0) last_mine = a + j;
+      }
+      const double scan = wave_scan_f64(own);
+      if (lane == 63) sums[wave] = scan;
+      __syncthreads();
+      double mine_at = base;
+#pragma unroll
+      for (int w = 0; w < VD_WAVES; w++) {
+        if (w < wave) mine_at += sums[w];
+        base += sums[w];
+      }
+      if (own > 0.0 && mine_at + scan > point) {
+        double run = mine_at + (scan - own);
+        int64_t here = p.V;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          run += x[j];
+          if (x[j] > 0.0 && run > point && here == p.V) here = a + j;
         }
-      // the walk's own rounding may leave it a hair short of the border that the scan has seen
-      if (here == p.V) here = last_mine;
+        // the walk's own rounding may leave it a hair short of the border that the scan has seen
+        if (here == p.V) here = last_mine;
+        atomicMin(reinterpret_cast<unsigned long long*>(&found), (unsigned long long)here);
+      }
+      __syncthreads();
+      if (found < p.V) break;             // the same for every thread
     }
-    if (here < p.V) atomicMin(reinterpret_cast<unsigned long long*>(&found), (unsigned long long)here);
-    if (last_mine >= 0) atomicMax(reinterpret_cast<long long*>(&last), (long long)last_mine);
-    __syncthreads();
+    if (found == p.V) {                   // no border: the chunk's last weight (256 atomics on one word cost 4 us: waves first)
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) {
+        const int64_t other = __shfl_xor((long long)last_mine, o, 64);
+        last_mine = other > last_mine ? other : last_mine;
+      }
+      if (lane == 0) atomicMax(reinterpret_cast<long long*>(&last), (long long)last_mine);
+      __syncthreads();
+    }
   }
   const int64_t token = found < p.V ? found : last;   // -1: the row holds no weight at all
   for (int i = tid; i <= p.K; i += VD_THREADS)
@@ -218,11 +244,14 @@ __global__ __launch_bounds__(VD_THREADS) void verify_draw_kernel(const VerifyArg
   if (tid == 0) p.accepted[r] = n;
 }
 
-// Chunks of a row: enough workgroups to keep the chip reading with few requests, at most one per lane of the wave that
-// scans their sums, and whole steps of 2048 elements.
-void pick_chunks(int64_t V, int& chunks, int& chunk_len) {
-  int64_t steps = (V + VD_STEP - 1) / VD_STEP;
-  const int64_t per = (steps + VD_MAX_CHUNKS - 1) / VD_MAX_CHUNKS;
+// Chunks of a row: about VD_TARGET workgroups over all rows (128 rows of 50257: 1024 workgroups 35 us, 4096 21, 8192 21), at most one per lane of the wave that scans their sums,
+// and whole steps of 2048 elements.
+constexpr int64_t VD_TARGET = 4096;
+void pick_chunks(int64_t R, int64_t V, int& chunks, int& chunk_len) {
+  const int64_t steps = (V + VD_STEP - 1) / VD_STEP;
+  int64_t want = (VD_TARGET + R - 1) / R;
+  if (want > VD_MAX_CHUNKS) want = VD_MAX_CHUNKS;
+  const int64_t per = (steps + want - 1) / want;
   chunk_len = (int)(per * VD_STEP);
   chunks = (int)((V + chunk_len - 1) / chunk_len);
 }
@@ -238,7 +267,7 @@ void launch(const VerifyArgs& a, int64_t R, hipStream_t s) {
 extern "C" int64_t mtp_verify_draft_workspace_bytes(int64_t R, int64_t V) {
   if (R <= 0 || V <= 0) return 0;
   int chunks, chunk_len;
-  pick_chunks(V, chunks, chunk_len);
+  pick_chunks(R, V, chunks, chunk_len);
   return R * chunks * 2 * (int64_t)sizeof(double);
 }
 
@@ -259,7 +288,7 @@ extern "C" int mtp_verify_draft(const int64_t* draft_tokens, const int64_t* draf
               (long long)need);
   VerifyArgs a = {draft_tokens, draft_lens, target_probs, draft_probs, uniforms, tokens, accepted,
                   static_cast<double*>(workspace), V, K, 0, 0};
-  pick_chunks(V, a.chunks, a.chunk_len);
+  pick_chunks(R, V, a.chunks, a.chunk_len);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == MTP_F32) launch<float>(a, R, s);
   else if (dtype == MTP_BF16) launch<uint16_t>(a, R, s);
