@@ -550,9 +550,12 @@ int mtp_qk_norm_rope_append(const void* qkv, const void* cos_table, const void* 
  * last new token is token kv_lens[r] - 1 of its cache, so row i of its n rows
  * sees the tokens up to kv_lens[r] - n + i:
  *   out[i,h,:] = softmax_t(scale * q[i,h,:] . K[t,h/g,:]) V[t,h/g,:]
- * with g = n_q_heads / n_kv_heads; a row that sees nothing gives zeros.  Any mix of single tokens, drafts and prompts.  Scores, softmax and
- * sums are fp32; probabilities are rounded to the tensor type for the product
- * with V.  Rows of no request are left as they were.  cu, kv_lens: int64 on the
+ * with g = n_q_heads / n_kv_heads; a row that sees nothing gives zeros.  Any
+ * mix of single tokens, drafts and prompts.  Scores, maximum and sums are fp32;
+ * probabilities are rounded to the tensor type for the product with V and
+ * summed as rounded (f16: times 2^11, so that those below 2^-14 of the largest
+ * keep their bits and only those below 2^-36 are lost).  Rows of no request are
+ * left as they were.  cu, kv_lens: int64 on the
  * device; kv_lens is clamped to the table row, cu to T.  Tokens whose page id is
  * outside the cache read as zeros.  What lies in a page behind a request's
  * length is not read into the result, whatever it holds; keys and values below
