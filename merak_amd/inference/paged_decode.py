@@ -25,8 +25,8 @@ class PagedLlamaDecoder:
     """``slots`` requests over ``n_pages`` pages of ``page_size`` tokens per layer.
 
     ``append(tokens, new_lens)`` adds ``new_lens[r]`` tokens to request r (host numbers; the tokens of all requests one
-    after the other) and returns the final-norm output of every new token.  A request that finds no page is refused:
-    ``self.granted[r]`` is False, its rows are meaningless and its state is as before.  ``release(r)`` gives a request's
+    after the other) and returns the final-norm output of every new token.  A request that finds no page, or whose length
+    would pass ``max_len``, is refused: ``self.granted[r]`` is False, its rows are meaningless and its state is as before.  ``release(r)`` gives a request's
     pages back.  ``q_norms`` / ``k_norms``: norm weights [head_dim] of each block's query and key heads, for models that
     have them."""
 
@@ -88,7 +88,10 @@ class PagedLlamaDecoder:
         if len(new_lens) != self.slots or min(new_lens) < 0 or tokens.shape != (T,):
             raise ValueError(f"append: {tuple(tokens.shape)} tokens for new_lens {new_lens} of {self.slots} requests")
         new = torch.tensor(new_lens, dtype=torch.int64).to(self._dev)
-        plan = ops.paged_plan(self.lens, new, self.held, self.block_tables, self.free_pages, self.free_count,
+        lens = self.lens
+        if self.max_len % self.page_size:     # the last page has room behind max_len, but the rotary tables end there
+            lens = torch.where(lens + new > self.max_len, -1, lens)      # a length that the plan refuses
+        plan = ops.paged_plan(lens, new, self.held, self.block_tables, self.free_pages, self.free_count,
                               self.page_size, T)
         self.held, self.free_count, self.granted = plan.held, plan.free_count, plan.granted
         self.lens = torch.where(plan.granted, self.lens + new, self.lens)
