@@ -81,8 +81,10 @@ class PagedLlamaDecoder:
         ops.paged_release(mask, self.held, self.block_tables, self.free_pages, self.free_count)
         self.lens.masked_fill_(mask, 0)
 
-    def append(self, tokens: torch.Tensor, new_lens: Sequence[int]) -> torch.Tensor:
-        """``tokens`` int64 [sum(new_lens)] -> hidden [sum(new_lens), H] after the final norm."""
+    def _run(self, tokens: torch.Tensor, new_lens: Sequence[int]):
+        """-> (hidden of the new tokens, plan, new_lens on the device).  Nothing of the decoder changes but table entries
+        behind the pages held and cache slots behind the lengths: a step that raises half way has not happened, and
+        ``_keep`` makes it count."""
         new_lens = [int(n) for n in new_lens]
         T = sum(new_lens)
         if len(new_lens) != self.slots or min(new_lens) < 0 or tokens.shape != (T,):
@@ -93,11 +95,9 @@ class PagedLlamaDecoder:
             lens = torch.where(lens + new > self.max_len, -1, lens)      # a length that the plan refuses
         plan = ops.paged_plan(lens, new, self.held, self.block_tables, self.free_pages, self.free_count,
                               self.page_size, T)
-        self.held, self.free_count, self.granted = plan.held, plan.free_count, plan.granted
-        self.lens = torch.where(plan.granted, self.lens + new, self.lens)
         x = ops.embedding_gather(tokens, self.embed, 0, self.embed.shape[0])
         if T == 0:
-            return x
+            return x, plan, new
         residual, most = None, max(new_lens)
         for i, w in enumerate(self.blocks):
             h, residual = ops.rmsnorm(x, w.input_norm, self.eps, residual, want_residual=True)
@@ -110,7 +110,18 @@ class PagedLlamaDecoder:
             h, residual = ops.rmsnorm(o, w.post_norm, self.eps, residual, want_residual=True)
             act = ops.linear_fwd(h, w.gate_up, None, ops.EPI_SWIGLU, want_pre=False)[1]
             x = ops.linear_fwd(act, w.down, None)[0]
-        return ops.rmsnorm(x, self.final_norm, self.eps, residual)
+        return ops.rmsnorm(x, self.final_norm, self.eps, residual), plan, new
+
+    def _keep(self, plan: ops.PagedPlan, new: torch.Tensor) -> None:
+        """The pages of a step that has run, and ``new[r]`` of its tokens, stay."""
+        self.held, self.free_count, self.granted = plan.held, plan.free_count, plan.granted
+        self.lens = torch.where(plan.granted, self.lens + new, self.lens)
+
+    def append(self, tokens: torch.Tensor, new_lens: Sequence[int]) -> torch.Tensor:
+        """``tokens`` int64 [sum(new_lens)] -> hidden [sum(new_lens), H] after the final norm."""
+        hidden, plan, new = self._run(tokens, new_lens)
+        self._keep(plan, new)
+        return hidden
 
     def logits(self, hidden: torch.Tensor) -> torch.Tensor:
         return ops.linear_fwd(hidden, self.lm_head, None)[0]
@@ -140,10 +151,9 @@ class PagedLlamaDecoder:
         if R != self.slots or last_tokens.shape != (R,):
             raise ValueError(f"verify: {tuple(last_tokens.shape)} tokens and {tuple(draft_tokens.shape)} drafts for "
                              f"{self.slots} requests")
-        before = self.lens
-        hidden = self.append(torch.cat([last_tokens[:, None], draft_tokens], 1).reshape(-1), [K + 1] * R)
+        hidden, plan, _ = self._run(torch.cat([last_tokens[:, None], draft_tokens], 1).reshape(-1), [K + 1] * R)
         z = ops.sample_top_k_top_p(self.logits(hidden), temperature, top_k, top_p, None, want_filtered=True)[1]
         tokens, accepted = ops.verify_draft(draft_tokens, torch.softmax(z, -1).view(R, K + 1, -1), draft_probs, uniforms)
         # rejected drafts leave the cache by the length alone: their slots are written again by the next tokens
-        self.lens = torch.where(self.granted, before + 1 + accepted, before)
+        self._keep(plan, 1 + accepted)
         return tokens, accepted

@@ -44,3 +44,32 @@ def test_a_request_ends_at_max_len(gpu, max_len, page_size):
     dec.append(text[0, :1].to(gpu), [1, 0])
     assert dec.granted.tolist() == [False, True] and dec.lens.tolist() == [max_len, 5]
     assert dec.held[0].item() == -(-max_len // page_size) and dec.free_count.item() <= free
+
+
+@pytest.mark.gpu
+def test_a_call_that_fails_leaves_the_state(gpu):
+    """Tokens of another type, uniforms of another shape, more drafts than the verification takes, a temperature of zero:
+    each raises, and the decoder goes on as if the call had not been made."""
+    m = model(gpu, 6)
+    text = torch.randint(0, V, (70,), generator=gen(1))
+    want = forward_fp32(m, text)
+    dec = decoder(on(gpu, m), slots=2)
+    dec.append(text[:21].to(gpu), [21, 0])
+    last, drafts, u = torch.zeros(2, dtype=torch.int64, device=gpu), torch.zeros(2, 3, dtype=torch.int64, device=gpu), \
+        torch.full((2, 4), 0.5, device=gpu)
+    many = torch.zeros(2, 65, dtype=torch.int64, device=gpu)
+    state = lambda: [t.clone() for t in (dec.lens, dec.held, dec.free_count, dec.granted)]
+    before = state()
+    for call in (lambda: dec.append(text[21:30].int().to(gpu), [9, 0]),
+                 lambda: dec.append(text[21:30], [9, 0]),                                   # not on the device
+                 lambda: dec.step(text[21:30].int().to(gpu), [9, 0]),
+                 lambda: dec.verify(last, drafts, u[:, :3]),
+                 lambda: dec.verify(last, drafts, u.double()),
+                 lambda: dec.verify(last, drafts, u, torch.zeros(2, 3, V - 1, device=gpu)),
+                 lambda: dec.verify(last, drafts, u, temperature=0.0),
+                 lambda: dec.verify(last, many, torch.full((2, 66), 0.5, device=gpu))):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            call()
+        assert all(torch.equal(a, b) for a, b in zip(before, state()))
+    out = dec.append(text[21:].to(gpu), [49, 0])
+    assert dec.granted.all() and rel(out, want[21:]) < 2e-2
