@@ -127,8 +127,8 @@ class PagedLlamaDecoder:
         return ops.linear_fwd(hidden, self.lm_head, None)[0]
 
     def step(self, tokens: torch.Tensor, new_lens: Sequence[int]) -> torch.Tensor:
-        """Greedy next token of every request that brought tokens (int64 [slots], -1 for the others): what the reference
-        picks at :223-227 from the last position."""
+        """Greedy next token of every request that brought tokens (int64 [slots], -1 for the others and for refused
+        ones): what the reference picks at :223-227 from the last position."""
         hidden = self.append(tokens, new_lens)
         last = torch.tensor(new_lens).cumsum(0) - 1
         who = [r for r, n in enumerate(new_lens) if n]
@@ -136,7 +136,7 @@ class PagedLlamaDecoder:
         if who:
             rows = hidden[last[who].to(self._dev)]
             out[torch.tensor(who).to(self._dev)] = ops.argmax_rows(self.logits(rows))
-        return out
+        return torch.where(self.granted, out, -1)
 
     def verify(self, last_tokens: torch.Tensor, draft_tokens: torch.Tensor, uniforms: torch.Tensor,
                draft_probs: Optional[torch.Tensor] = None, temperature: float = 1.0, top_k: int = 0, top_p: float = 0.0
@@ -146,7 +146,7 @@ class PagedLlamaDecoder:
         target's probabilities, and ``ops.verify_draft`` decides.  -> (tokens [slots, K + 1], accepted [slots]); the
         cache keeps ``last_tokens`` and the accepted drafts, the last of ``tokens`` is the next call's ``last_tokens``.
         ``draft_probs`` fp32 [slots, K, V], or None for drafts without probabilities of their own; ``uniforms`` fp32
-        [slots, K + 1]."""
+        [slots, K + 1].  A refused request (``self.granted[r]`` False) has only -1 and 0 accepted."""
         R, K = draft_tokens.shape
         if R != self.slots or last_tokens.shape != (R,):
             raise ValueError(f"verify: {tuple(last_tokens.shape)} tokens and {tuple(draft_tokens.shape)} drafts for "
@@ -156,4 +156,4 @@ class PagedLlamaDecoder:
         tokens, accepted = ops.verify_draft(draft_tokens, torch.softmax(z, -1).view(R, K + 1, -1), draft_probs, uniforms)
         # rejected drafts leave the cache by the length alone: their slots are written again by the next tokens
         self._keep(plan, 1 + accepted)
-        return tokens, accepted
+        return torch.where(plan.granted[:, None], tokens, -1), torch.where(plan.granted, accepted, 0)

@@ -73,3 +73,28 @@ def test_a_call_that_fails_leaves_the_state(gpu):
         assert all(torch.equal(a, b) for a, b in zip(before, state()))
     out = dec.append(text[21:].to(gpu), [49, 0])
     assert dec.granted.all() and rel(out, want[21:]) < 2e-2
+
+
+@pytest.mark.gpu
+def test_refused_requests_give_no_tokens(gpu):
+    """A pool too small for one request, then a request at max_len: step and verify say -1 and 0 for them, and the others
+    get what a decoder without them gives."""
+    m = on(gpu, model(gpu, 7))
+    g = gen(3)
+    text = torch.randint(0, V, (2, 40), generator=g).to(gpu)
+    dec, alone = decoder(m, slots=2, n_pages=4), decoder(m, slots=1, n_pages=4)
+    got = dec.step(torch.cat([text[0], text[1]]), [40, 40])               # three pages each, four in the pool
+    assert dec.granted.tolist() == [True, False]
+    want = alone.step(text[0], [40])
+    assert got.tolist() == [want.item(), -1]
+    drafts, u = torch.randint(0, V, (2, 12), generator=g).to(gpu), torch.rand(2, 13, generator=g).to(gpu)
+    tokens, n = dec.verify(torch.stack([want[0], want[0]]), drafts, u, top_k=1)
+    assert dec.granted.tolist() == [True, False] and n[1].item() == 0 and (tokens[1] == -1).all() and dec.lens[1].item() == 0
+    t1, n1 = alone.verify(want, drafts[:1], u[:1], top_k=1)
+    assert torch.equal(tokens[0], t1[0]) and n[0].item() == n1.item() and dec.lens[0].item() == alone.lens.item()
+    full = decoder(m, slots=2, max_len=42)
+    full.append(torch.cat([text[0], text[1, :3]]), [40, 3])
+    tokens, n = full.verify(text[:, 0], drafts[:, :3], u[:, :4], top_k=1)
+    assert full.granted.tolist() == [False, True] and (tokens[0] == -1).all() and n[0].item() == 0
+    assert full.lens.tolist() == [40, 3 + 1 + n[1].item()]
+    assert full.step(text[:, 0].repeat_interleave(torch.tensor([3, 1], device=gpu)), [3, 1])[0].item() == -1
