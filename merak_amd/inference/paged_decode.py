@@ -81,8 +81,9 @@ class PagedLlamaDecoder:
         ops.paged_release(mask, self.held, self.block_tables, self.free_pages, self.free_count)
         self.lens.masked_fill_(mask, 0)
 
-    def _run(self, tokens: torch.Tensor, new_lens: Sequence[int]):
-        """-> (hidden of the new tokens, plan, new_lens on the device).  Nothing of the decoder changes but table entries
+    def _run(self, tokens: torch.Tensor, new_lens: Sequence[int], takes: Optional[torch.Tensor] = None):
+        """-> (hidden of the new tokens, plan, new_lens on the device).  ``takes`` bool [slots] on the device: False: the
+        slot's tokens are computed for nothing (the plan refuses them).  Nothing of the decoder changes but table entries
         behind the pages held and cache slots behind the lengths: a step that raises half way has not happened, and
         ``_keep`` makes it count."""
         new_lens = [int(n) for n in new_lens]
@@ -93,6 +94,8 @@ class PagedLlamaDecoder:
         lens = self.lens
         if self.max_len % self.page_size:     # the last page has room behind max_len, but the rotary tables end there
             lens = torch.where(lens + new > self.max_len, -1, lens)      # a length that the plan refuses
+        if takes is not None:
+            lens = torch.where(takes, lens, -1)
         plan = ops.paged_plan(lens, new, self.held, self.block_tables, self.free_pages, self.free_count,
                               self.page_size, T)
         x = ops.embedding_gather(tokens, self.embed, 0, self.embed.shape[0])
@@ -139,21 +142,46 @@ class PagedLlamaDecoder:
         return torch.where(self.granted, out, -1)
 
     def verify(self, last_tokens: torch.Tensor, draft_tokens: torch.Tensor, uniforms: torch.Tensor,
-               draft_probs: Optional[torch.Tensor] = None, temperature: float = 1.0, top_k: int = 0, top_p: float = 0.0
-               ) -> Tuple[torch.Tensor, torch.Tensor]:
-        """One step of speculative decoding for all requests: ``last_tokens`` int64 [slots] (not yet in the cache) and
-        ``draft_tokens`` int64 [slots, K] go through the model together, the sampling tail's filter and softmax give the
-        target's probabilities, and ``ops.verify_draft`` decides.  -> (tokens [slots, K + 1], accepted [slots]); the
-        cache keeps ``last_tokens`` and the accepted drafts, the last of ``tokens`` is the next call's ``last_tokens``.
+               draft_probs: Optional[torch.Tensor] = None, temperature: float = 1.0, top_k: int = 0, top_p: float = 0.0,
+               draft_lens: Optional[Sequence[int]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """One step of speculative decoding: ``last_tokens`` int64 [slots] (not yet in the cache) and ``draft_tokens``
+        int64 [slots, K] go through the model together, the sampling tail's filter and softmax give the target's
+        probabilities, and ``ops.verify_draft`` decides.  -> (tokens [slots, K + 1], accepted [slots]); the cache keeps
+        ``last_tokens`` and the accepted drafts, the last of ``tokens`` is the next call's ``last_tokens``.
         ``draft_probs`` fp32 [slots, K, V], or None for drafts without probabilities of their own; ``uniforms`` fp32
-        [slots, K + 1].  A refused request (``self.granted[r]`` False) has only -1 and 0 accepted."""
+        [slots, K + 1].
+
+        ``draft_lens`` (host numbers) says how many drafts each request has, 0 .. K, or -1 for a slot that is left out;
+        a request near ``max_len`` or a full pool can ask for fewer.  None: K drafts for every slot that holds tokens;
+        empty slots (never used, or released) are left out, though their rows are computed.  Slots that are left out and
+        refused requests (``self.granted[r]`` False) have only -1 and 0 accepted, and stay as they are."""
         R, K = draft_tokens.shape
         if R != self.slots or last_tokens.shape != (R,):
             raise ValueError(f"verify: {tuple(last_tokens.shape)} tokens and {tuple(draft_tokens.shape)} drafts for "
                              f"{self.slots} requests")
-        hidden, plan, _ = self._run(torch.cat([last_tokens[:, None], draft_tokens], 1).reshape(-1), [K + 1] * R)
+        tokens = torch.cat([last_tokens[:, None], draft_tokens], 1).reshape(-1)
+        if draft_lens is None:
+            takes, limits, rows = self.lens > 0, None, None
+            hidden, plan, _ = self._run(tokens, [K + 1] * R, takes)
+        else:
+            draft_lens = [int(n) for n in draft_lens]
+            if len(draft_lens) != R or min(draft_lens) < -1 or max(draft_lens) > K:
+                raise ValueError(f"verify: draft_lens {draft_lens} for {R} requests of {K} drafts")
+            limits = torch.tensor(draft_lens, dtype=torch.int64).to(self._dev)
+            takes = limits >= 0
+            rows = torch.tensor([r * (K + 1) + i for r, n in enumerate(draft_lens) for i in range(n + 1)],
+                                dtype=torch.int64).to(self._dev)
+            hidden, plan, _ = self._run(tokens[rows], [n + 1 for n in draft_lens])
+        if hidden.shape[0] == 0:
+            self._keep(plan, torch.zeros_like(self.lens))
+            return torch.full_like(tokens, -1).view(R, K + 1), torch.zeros_like(self.lens)
         z = ops.sample_top_k_top_p(self.logits(hidden), temperature, top_k, top_p, None, want_filtered=True)[1]
-        tokens, accepted = ops.verify_draft(draft_tokens, torch.softmax(z, -1).view(R, K + 1, -1), draft_probs, uniforms)
+        probs = torch.softmax(z, -1)
+        if rows is not None and rows.shape[0] < R * (K + 1):      # rows of drafts that are not there: no weight
+            probs = torch.zeros((R * (K + 1), probs.shape[1]), dtype=probs.dtype, device=self._dev).index_copy_(0, rows, probs)
+        tokens, accepted = ops.verify_draft(draft_tokens, probs.view(R, K + 1, -1), draft_probs, uniforms, limits)
+        served = plan.granted & takes
         # rejected drafts leave the cache by the length alone: their slots are written again by the next tokens
-        self._keep(plan, 1 + accepted)
-        return torch.where(plan.granted[:, None], tokens, -1), torch.where(plan.granted, accepted, 0)
+        self._keep(plan, torch.where(served, 1 + accepted, 0))
+        self.granted = plan.granted | ~takes
+        return torch.where(served[:, None], tokens, -1), torch.where(served, accepted, 0)

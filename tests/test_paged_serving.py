@@ -82,14 +82,15 @@ def test_refused_requests_give_no_tokens(gpu):
     m = on(gpu, model(gpu, 7))
     g = gen(3)
     text = torch.randint(0, V, (2, 40), generator=g).to(gpu)
-    dec, alone = decoder(m, slots=2, n_pages=4), decoder(m, slots=1, n_pages=4)
-    got = dec.step(torch.cat([text[0], text[1]]), [40, 40])               # three pages each, four in the pool
+    dec, alone = decoder(m, slots=2, n_pages=5), decoder(m, slots=1, n_pages=5)
+    got = dec.step(torch.cat([text[0], text[1]]), [40, 40])               # three pages each, five in the pool
     assert dec.granted.tolist() == [True, False]
     want = alone.step(text[0], [40])
     assert got.tolist() == [want.item(), -1]
     drafts, u = torch.randint(0, V, (2, 12), generator=g).to(gpu), torch.rand(2, 13, generator=g).to(gpu)
+    dec.append(text[1, :5], [0, 5])                                       # one page; the last one goes to the first request
     tokens, n = dec.verify(torch.stack([want[0], want[0]]), drafts, u, top_k=1)
-    assert dec.granted.tolist() == [True, False] and n[1].item() == 0 and (tokens[1] == -1).all() and dec.lens[1].item() == 0
+    assert dec.granted.tolist() == [True, False] and n[1].item() == 0 and (tokens[1] == -1).all() and dec.lens[1].item() == 5
     t1, n1 = alone.verify(want, drafts[:1], u[:1], top_k=1)
     assert torch.equal(tokens[0], t1[0]) and n[0].item() == n1.item() and dec.lens[0].item() == alone.lens.item()
     full = decoder(m, slots=2, max_len=42)
@@ -98,3 +99,69 @@ def test_refused_requests_give_no_tokens(gpu):
     assert full.granted.tolist() == [False, True] and (tokens[0] == -1).all() and n[0].item() == 0
     assert full.lens.tolist() == [40, 3 + 1 + n[1].item()]
     assert full.step(text[:, 0].repeat_interleave(torch.tensor([3, 1], device=gpu)), [3, 1])[0].item() == -1
+
+
+@pytest.mark.gpu
+def test_verify_leaves_idle_slots_alone(gpu):
+    """A slot that was never used in front of the running one, and a released one behind it: they take no pages (the pool
+    has none to spare), keep length 0 and start from nothing afterwards; the running request gets what it gets alone."""
+    mc = model(gpu, 8)
+    m = on(gpu, mc)
+    g = gen(4)
+    text = torch.randint(0, V, (3, 30), generator=g)
+    dec, alone = decoder(m, slots=3, n_pages=5), decoder(m, slots=1, n_pages=3)
+    dec.append(torch.cat([text[1], text[2]]).to(gpu), [0, 30, 30])
+    dec.release([2])
+    alone.append(text[1].to(gpu), [30])
+    last = torch.tensor([3, 5, 7], device=gpu)
+    for k in range(3):
+        drafts, u = torch.randint(0, V, (3, 4), generator=g).to(gpu), torch.rand(3, 5, generator=g).to(gpu)
+        tokens, n = dec.verify(last, drafts, u, top_k=1)
+        t1, n1 = alone.verify(last[1:2], drafts[1:2], u[1:2], top_k=1)
+        assert torch.equal(tokens[1], t1[0]) and n.tolist() == [0, n1.item(), 0]
+        assert (tokens[0] == -1).all() and (tokens[2] == -1).all() and dec.granted.all()
+        assert dec.lens.tolist() == [0, alone.lens.item(), 0] and dec.held.tolist() == [0, alone.held.item(), 0]
+        last = torch.where(tokens >= 0, tokens, 0).gather(1, n[:, None]).squeeze(1)
+    out = dec.append(text[2, :20].to(gpu), [0, 0, 20])
+    assert dec.granted.all() and rel(out, forward_fp32(mc, text[2])[:20]) < 2e-2
+
+
+@pytest.mark.gpu
+def test_verify_with_drafts_of_different_lengths(gpu):
+    """No slots, some drafts, none, all of them: each request gets what it gets alone with that many; slots left out stay,
+    an empty slot that is named takes part, and a request that ends at max_len finishes with the drafts that fit."""
+    m = on(gpu, model(gpu, 9))
+    g = gen(5)
+    K, text = 4, torch.randint(0, V, (4, 25), generator=g).to(gpu)
+    lens = [25, 11, 0, 20]
+    dec = decoder(m, slots=4, max_len=27, n_pages=8)
+    dec.append(torch.cat([text[r, :n] for r, n in enumerate(lens)]), lens)
+    drafts, u = torch.randint(0, V, (4, K), generator=g).to(gpu), torch.rand(4, K + 1, generator=g).to(gpu)
+    guess = torch.softmax(torch.randn(4, K, V, generator=g) * 3, -1).to(gpu)
+    last = text[:, 3]
+    tokens, n = dec.verify(last, drafts, u, draft_lens=[-1] * 4)
+    assert (tokens == -1).all() and not n.any() and dec.lens.tolist() == lens and dec.granted.all()
+    tokens, n = dec.verify(last, drafts, u, draft_lens=[K, -1, -1, -1])   # five tokens where two fit
+    assert dec.granted.tolist() == [False, True, True, True] and (tokens == -1).all() and dec.lens.tolist() == lens
+    for probs in (None, guess):
+        want = [1, K, 0, -1]
+        before = dec.lens.tolist()
+        tokens, n = dec.verify(last, drafts, u, probs, top_k=1, draft_lens=want)
+        after = dec.lens.tolist()
+        for r in range(4):
+            if want[r] < 0:
+                assert (tokens[r] == -1).all() and n[r].item() == 0 and after[r] == before[r]
+                continue
+            one = decoder(m, slots=1, max_len=27)
+            if lens[r]:
+                one.append(text[r, :lens[r]], [lens[r]])
+            k = want[r]
+            t1, n1 = one.verify(last[r:r + 1], drafts[r:r + 1, :k], torch.cat([u[r:r + 1, :k], u[r:r + 1, K:]], 1),
+                                None if probs is None else probs[r:r + 1, :k], top_k=1, draft_lens=[k])
+            assert dec.granted[r] and n[r].item() == n1.item() <= k and after[r] == before[r] + 1 + n1.item()
+            assert tokens[r].tolist() == t1[0].tolist() + [-1] * (K - k)
+        dec.release(range(4))
+        dec.append(torch.cat([text[r, :n] for r, n in enumerate(lens)]), lens)
+    for bad in ([K + 1, 0, 0, 0], [0, 0, 0], [-2, 0, 0, 0]):
+        with pytest.raises(ValueError, match="draft_lens"):
+            dec.verify(last, drafts, u, draft_lens=bad)
