@@ -39,10 +39,25 @@ class PagedLlamaDecoder:
         self.embed, self.blocks, self.final_norm, self.lm_head = embed, blocks, final_norm, lm_head
         self.n_q, self.n_kv, self.head_dim, self.eps = n_q_heads, n_kv_heads, head_dim, eps
         self.max_len, self.slots, self.page_size = max_len, slots, page_size
+        # what the operators of a step would refuse only after pages have been handed out
+        if dt not in (torch.bfloat16, torch.float16) or head_dim not in (64, 128):
+            raise ValueError(f"head_dim must be 64 or 128 and the weights bf16 or f16, got {head_dim} and {dt}")
+        if n_kv_heads < 1 or n_q_heads < 1 or n_q_heads % n_kv_heads:
+            raise ValueError(f"{n_q_heads} query heads for {n_kv_heads} key heads")
+        if page_size < 16 or page_size & (page_size - 1):
+            raise ValueError(f"page_size must be a power of two of at least 16, got {page_size}")
+        if max_len < 1 or not 1 <= slots <= 4096 or (n_pages is not None and n_pages < 1):
+            raise ValueError(f"max_len {max_len}, slots {slots} (1 .. 4096), n_pages {n_pages}")
         self.q_norms = list(q_norms) if q_norms is not None else [None] * len(blocks)
         self.k_norms = list(k_norms) if k_norms is not None else [None] * len(blocks)
         if len(self.q_norms) != len(blocks) or len(self.k_norms) != len(blocks):
             raise ValueError("q_norms and k_norms need one entry per block")
+        for i, (w, *norms) in enumerate(zip(blocks, self.q_norms, self.k_norms)):
+            if w.qkv.shape[0] != (n_q_heads + 2 * n_kv_heads) * head_dim or w.o.shape[1] != n_q_heads * head_dim:
+                raise ValueError(f"block {i}: weights {tuple(w.qkv.shape)} and {tuple(w.o.shape)} for {n_q_heads}+2*"
+                                 f"{n_kv_heads} heads of {head_dim}")
+            if any(n is not None and (n.shape != (head_dim,) or n.dtype != dt) for n in norms):
+                raise ValueError(f"block {i}: head norms must be {dt} [{head_dim}]")
         per_request = -(-max_len // page_size)
         n_pages = slots * per_request if n_pages is None else n_pages
         cache = lambda: torch.zeros((n_pages, n_kv_heads, page_size, head_dim), dtype=dt, device=dev)
