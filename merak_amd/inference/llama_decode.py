@@ -58,6 +58,89 @@ class LlamaBlockWeights:
     down: torch.Tensor         # [H, I]
 
 
+def _is_plain_rmsnorm(norm: torch.nn.Module, eps: float) -> bool:
+    """Whether the module computes weight * x / sqrt(mean(x^2) + eps), by what it gives for small rows (where eps counts);
+    a norm that scales by 1 + weight, subtracts the mean or has another eps does not."""
+    w = norm.weight.data
+    x = torch.linspace(-1.0, 2.0, w.numel(), device=w.device) * (2.0 * eps) ** 0.5
+    x = torch.stack([x, x.flip(0)]).to(w.dtype)
+    want = w.float() * x.float() * torch.rsqrt(x.float().square().mean(-1, keepdim=True) + eps)
+    with torch.no_grad():
+        got = norm(x).float()
+    # two roundings to the weight's type; another eps (a factor of 10) or scale is off by tens of per cent
+    return bool(((got - want).norm() <= 0.02 * want.norm()).item())
+
+
+def hf_weights(model, max_len: int, head_norms: bool = False):
+    """Weights and numbers of a ``transformers`` causal model of Llama's arithmetic -> (embed, blocks, final norm, LM head,
+    query heads, key heads, head_dim, eps, rope theta, rope scaling, query norms, key norms); the norms of the query and key
+    heads are None per block unless ``head_norms``.  Raises ValueError for a model that computes something else with
+    modules of the same names: biases, other norms, activations, scales or masks."""
+    cfg = model.config
+    eps = cfg.rms_norm_eps
+    head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
+
+    def refuse(what):
+        raise ValueError(f"{type(model).__name__}: {what}; the decoder computes Llama's blocks only")
+
+    if cfg.hidden_act not in ("silu", "swish"):
+        refuse(f"activation {cfg.hidden_act}")
+    for name in ("embedding_multiplier", "residual_multiplier", "logits_scaling", "partial_rotary_factor"):
+        if getattr(cfg, name, None) not in (None, 1, 1.0):
+            refuse(f"{name} {getattr(cfg, name)}")
+    window = getattr(cfg, "sliding_window", None) if getattr(cfg, "use_sliding_window", True) else None
+    if window is not None and window < max_len and "sliding_attention" in (getattr(cfg, "layer_types", None) or ["sliding_attention"]):
+        refuse(f"a sliding window of {window} for up to {max_len} tokens")
+    extra = {n for n, _ in model.model.named_children()} - {"embed_tokens", "layers", "norm", "rotary_emb"}
+    if extra:
+        refuse(f"the model has {', '.join(sorted(extra))}")
+    known = {"": {"self_attn", "mlp", "input_layernorm", "post_attention_layernorm"},
+             "self_attn": {"q_proj", "k_proj", "v_proj", "o_proj", "rotary_emb"} | ({"q_norm", "k_norm"} if head_norms else set()),
+             "mlp": {"gate_proj", "up_proj", "down_proj", "act_fn"}}
+    blocks, q_norms, k_norms, norms = [], [], [], [("norm", model.model.norm)]
+    for i, layer in enumerate(model.model.layers):
+        a, m = layer.self_attn, layer.mlp
+        for part, names in known.items():
+            extra = {n for n, _ in (getattr(layer, part) if part else layer).named_children()} - names
+            if extra:
+                refuse(f"layer {i} has {', '.join(sorted(extra))}")
+        for name, proj in (("q_proj", a.q_proj), ("k_proj", a.k_proj), ("v_proj", a.v_proj), ("o_proj", a.o_proj),
+                           ("gate_proj", m.gate_proj), ("up_proj", m.up_proj), ("down_proj", m.down_proj)):
+            if getattr(proj, "bias", None) is not None:
+                refuse(f"layer {i}: {name} has a bias")
+        if abs(getattr(a, "scaling", head_dim ** -0.5) * head_dim ** 0.5 - 1) > 1e-6:
+            refuse(f"layer {i}: scores scaled by {a.scaling}")
+        if not getattr(a, "use_rope", True):
+            refuse(f"layer {i} without rotary embedding")
+        blocks.append(LlamaBlockWeights(
+            layer.input_layernorm.weight.data,
+            torch.cat([a.q_proj.weight.data, a.k_proj.weight.data, a.v_proj.weight.data]).contiguous(),
+            a.o_proj.weight.data.contiguous(), layer.post_attention_layernorm.weight.data,
+            torch.cat([m.gate_proj.weight.data, m.up_proj.weight.data]).contiguous(),
+            m.down_proj.weight.data.contiguous()))
+        norms += [(f"layer {i}: input_layernorm", layer.input_layernorm),
+                  (f"layer {i}: post_attention_layernorm", layer.post_attention_layernorm)]
+        for name, into in (("q_norm", q_norms), ("k_norm", k_norms)):
+            norm = getattr(a, name, None)
+            into.append(None if norm is None else norm.weight.data)
+            if norm is not None:
+                norms.append((f"layer {i}: {name}", norm))
+                if norm.weight.shape != (head_dim,):
+                    refuse(f"layer {i}: {name} of {tuple(norm.weight.shape)} for heads of {head_dim}")
+    for name, norm in norms:
+        if getattr(norm, "bias", None) is not None or not _is_plain_rmsnorm(norm, eps):
+            refuse(f"{name} is not weight * x / sqrt(mean(x^2) + {eps})")
+    if getattr(model.lm_head, "bias", None) is not None:
+        refuse("lm_head has a bias")
+    rp = getattr(cfg, "rope_parameters", None) or getattr(cfg, "rope_scaling", None) or {}
+    if rp.get("partial_rotary_factor", 1.0) != 1.0:
+        refuse(f"partial_rotary_factor {rp['partial_rotary_factor']}")
+    theta = rp.get("rope_theta", getattr(cfg, "rope_theta", 10000.0))
+    scaling = rp if rp.get("rope_type", "default") != "default" else None
+    return (model.model.embed_tokens.weight.data, blocks, model.model.norm.weight.data, model.lm_head.weight.data,
+            cfg.num_attention_heads, cfg.num_key_value_heads, head_dim, eps, theta, scaling, q_norms, k_norms)
+
+
 class LlamaDecoder:
     """Decode-only runner: ``step(tokens)`` appends one token per sequence and returns the next one.
 
@@ -94,24 +177,10 @@ class LlamaDecoder:
 
     @classmethod
     def from_hf(cls, model, max_len: int = 4096, batch: int = 1, fused: Optional[bool] = None):
-        """From a ``transformers`` ``LlamaForCausalLM`` (weights are concatenated once, not shared)."""
-        cfg = model.config
-        blocks = []
-        for layer in model.model.layers:
-            a, m = layer.self_attn, layer.mlp
-            blocks.append(LlamaBlockWeights(
-                layer.input_layernorm.weight.data,
-                torch.cat([a.q_proj.weight.data, a.k_proj.weight.data, a.v_proj.weight.data]).contiguous(),
-                a.o_proj.weight.data.contiguous(), layer.post_attention_layernorm.weight.data,
-                torch.cat([m.gate_proj.weight.data, m.up_proj.weight.data]).contiguous(),
-                m.down_proj.weight.data.contiguous()))
-        rp = getattr(cfg, "rope_parameters", None) or getattr(cfg, "rope_scaling", None) or {}
-        theta = rp.get("rope_theta", getattr(cfg, "rope_theta", 10000.0))
-        scaling = rp if rp.get("rope_type", "default") != "default" else None
-        head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
-        return cls(model.model.embed_tokens.weight.data, blocks, model.model.norm.weight.data,
-                   model.lm_head.weight.data, cfg.num_attention_heads, cfg.num_key_value_heads, head_dim,
-                   cfg.rms_norm_eps, theta, scaling, max_len, batch, fused)
+        """From a ``transformers`` ``LlamaForCausalLM`` (weights are concatenated once, not shared), or a model of the same
+        arithmetic; others are refused (``hf_weights``)."""
+        embed, blocks, norm, head, n_q, n_kv, head_dim, eps, theta, scaling = hf_weights(model, max_len)[:10]
+        return cls(embed, blocks, norm, head, n_q, n_kv, head_dim, eps, theta, scaling, max_len, batch, fused)
 
     def reset(self):
         self.lens.zero_()

@@ -18,7 +18,7 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 
 from .. import ops
-from .llama_decode import LlamaBlockWeights, LlamaDecoder, rope_tables
+from .llama_decode import LlamaBlockWeights, hf_weights, rope_tables
 
 
 class PagedLlamaDecoder:
@@ -75,18 +75,13 @@ class PagedLlamaDecoder:
 
     @classmethod
     def from_hf(cls, model, **kw):
-        """From a ``transformers`` Llama-shaped causal model (weights as ``LlamaDecoder.from_hf`` lays them out); norms of
-        the query and key heads are taken where its attention has ``q_norm`` / ``k_norm``."""
-        base = LlamaDecoder.from_hf(model, max_len=1, batch=1)
-        cfg = model.config
-        rp = getattr(cfg, "rope_parameters", None) or getattr(cfg, "rope_scaling", None) or {}
-        layers = [layer.self_attn for layer in model.model.layers]
-        if hasattr(layers[0], "q_norm"):
-            kw.setdefault("q_norms", [a.q_norm.weight.data for a in layers])
-            kw.setdefault("k_norms", [a.k_norm.weight.data for a in layers])
-        return cls(base.embed, base.blocks, base.final_norm, base.lm_head, base.n_q, base.n_kv, base.head_dim, base.eps,
-                   rp.get("rope_theta", getattr(cfg, "rope_theta", 10000.0)),
-                   rp if rp.get("rope_type", "default") != "default" else None, **kw)
+        """From a ``transformers`` causal model of Llama's arithmetic (``hf_weights`` refuses others), with norms of the query
+        and key heads where its attention has them; ``kw``: the sizes of the cache."""
+        embed, blocks, norm, head, n_q, n_kv, head_dim, eps, theta, scaling, q_norms, k_norms = hf_weights(
+            model, kw.get("max_len", 4096), head_norms=True)
+        kw.setdefault("q_norms", q_norms)
+        kw.setdefault("k_norms", k_norms)
+        return cls(embed, blocks, norm, head, n_q, n_kv, head_dim, eps, theta, scaling, **kw)
 
     def release(self, finished: Sequence[int]) -> None:
         """The pages of these requests go back to the pool; their lengths become 0."""
