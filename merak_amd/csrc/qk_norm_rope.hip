@@ -410,7 +410,7 @@ int check_common(const char* what, const RotArgs& a, int head_dim, int table_dty
   MTP_REQUIRE(a.tokens >= 0 && a.n_q > 0 && a.n_kv > 0 && a.n_q <= 4096 && a.n_kv <= 4096 && a.max_positions > 0,
               MTP_EINVAL, "%s: T=%lld heads %d/%d max_positions=%lld", what, (long long)a.tokens, a.n_q, a.n_kv,
               (long long)a.max_positions);
-  MTP_REQUIRE(a.tokens <= 0x7fffffffll / 1024, MTP_EUNSUPPORTED, "%s: T=%lld (at most 2^21)", what, (long long)a.tokens);
+  MTP_REQUIRE(a.tokens <= 1ll << 21, MTP_EUNSUPPORTED, "%s: T=%lld (at most 2^21)", what, (long long)a.tokens);
   MTP_REQUIRE(a.tokens == 0 || (a.qkv && a.cos_t && a.sin_t && a.positions), MTP_EINVAL, "%s: null pointer", what);
   MTP_REQUIRE(((uintptr_t)a.qkv | (uintptr_t)a.cos_t | (uintptr_t)a.sin_t | (uintptr_t)a.q_weight |
                (uintptr_t)a.k_weight | (uintptr_t)a.q_out | (uintptr_t)a.k_out | (uintptr_t)a.k_cache |

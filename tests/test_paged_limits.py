@@ -59,3 +59,38 @@ def test_attn_paged_keeps_a_flat_tail(gpu, dtype, d, hq, new, requests, log2p):
     bound = half * ref.abs() * 1.01 + step + half * mass * 1.02 + 2 * tiny + (2 * n + 64 + 8 * x) * U32 * mass
     ratio = (got - ref).abs() / bound
     assert not torch.isnan(got).any() and ratio.max() <= 1, (float(ratio.max()), got[0, 0, 0, :2], ref[0, 0, :2])
+
+
+# --------------------------------------------------------------------------- the most tokens of a call
+def test_qk_norm_rope_token_limit():
+    """2^21 rows are taken, one more is not (the null pointer is what a call of 2^21 is refused for here)."""
+    from merak_amd import _lib
+    lib, A = _lib.lib(), 4096
+    calls = (lambda T: lib.mtp_qk_norm_rope(None, A, A, 0, A, None, None, A, A, T, 1, 1, 64, 10, 1e-6, 1, None),
+             lambda T: lib.mtp_qk_norm_rope_append(None, A, A, 0, A, A, None, None, A, A, A, T, 1, 1, 64, 10, 4, 16, 1e-6, 1, None),
+             lambda T: lib.mtp_qk_norm_rope_bwd(A, A, A, None, A, A, 0, A, None, None, A, None, None, None, 0, T, 1, 1, 64, 10,
+                                                1e-6, 1, None))
+    for call in calls:
+        assert call(2 ** 21) == -1 and b"null" in lib.mtp_last_error()
+        assert call(2 ** 21 + 1) == -2 and b"2^21" in lib.mtp_last_error()
+
+
+@pytest.mark.gpu
+def test_qk_norm_rope_of_the_most_tokens(gpu):
+    """2^21 rows, forward and backward: the last rows equal those of a small call on the same data."""
+    T, d, few = 2 ** 21, 64, 300
+    qkv = torch.randn(few, 3 * d, generator=gen(1)).half().to(gpu)
+    cos, sin = (torch.randn(50, d, generator=gen(i)).to(gpu) for i in (2, 3))
+    pos = torch.randint(0, 50, (few,), generator=gen(4)).to(gpu)
+    w = (torch.rand(d, generator=gen(5)) + 0.5).half().to(gpu)
+    up = [torch.randn(few, 1, d, generator=gen(6 + i)).half().to(gpu) for i in range(3)]
+    big = lambda t: torch.cat([torch.zeros((T - few, *t.shape[1:]), dtype=t.dtype, device=gpu), t])
+    q, k = ops.qk_norm_rope(big(qkv), cos, sin, big(pos), 1, w, w)
+    q1, k1 = ops.qk_norm_rope(qkv, cos, sin, pos, 1, w, w)
+    assert torch.equal(q[-few:], q1) and torch.equal(k[-few:], k1) and not q[:-few].any()
+    dqkv, dqw, dkw = ops.qk_norm_rope_bwd(*[big(u) for u in up], big(qkv), cos, sin, big(pos), w, w)
+    d1, w1, w2 = ops.qk_norm_rope_bwd(*up, qkv, cos, sin, pos, w, w)
+    assert torch.equal(dqkv[-few:], d1) and not dqkv[:-few].any()
+    # the same terms, added up in another order: 2^-11 for the result's rounding on either side and the fp32 sums' own
+    for a, b in ((dqw, w1), (dkw, w2)):
+        assert ((a.double() - b.double()).abs() <= 2 * 2.0 ** -11 * b.double().abs() * 1.01 + 1e-3).all()
