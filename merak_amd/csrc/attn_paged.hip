@@ -830,7 +830,7 @@ extern "C" int mtp_attn_paged(const void* q, const void* k_cache, const void* v_
   MTP_REQUIRE(head_dim == 64 || head_dim == 128, MTP_EUNSUPPORTED, "attn_paged: head_dim %d (64 or 128)", head_dim);
   MTP_REQUIRE(n_q_heads > 0 && n_kv_heads > 0 && n_q_heads % n_kv_heads == 0 && n_q_heads <= 4096, MTP_EINVAL,
               "attn_paged: heads %d/%d", n_q_heads, n_kv_heads);
-  MTP_REQUIRE(T >= 0 && T * n_q_heads <= 0x3fffffffll && requests >= 0 && requests <= 0x7fffff, MTP_EINVAL,
+  MTP_REQUIRE(T >= 0 && T <= 0x3fffffffll / n_q_heads && requests >= 0 && requests <= 0x7fffff, MTP_EINVAL,
               "attn_paged: T=%lld requests=%lld", (long long)T, (long long)requests);
   MTP_REQUIRE(page_size >= AP_PAGE_MIN && (page_size & (page_size - 1)) == 0, MTP_EUNSUPPORTED,
               "attn_paged: page_size=%lld (a power of two, at least %d)", (long long)page_size, AP_PAGE_MIN);

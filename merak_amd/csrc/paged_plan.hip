@@ -231,7 +231,7 @@ extern "C" int mtp_paged_plan(const int64_t* lens, const int64_t* new_lens, cons
                               int64_t free_capacity, int64_t tokens, void* stream) {
   const int rc = check_sizes("paged_plan", requests, max_pages, free_capacity);
   if (rc) return rc;
-  MTP_REQUIRE(page_size >= 1 && (page_size & (page_size - 1)) == 0 && max_pages * page_size <= 0x7fffffffll, MTP_EINVAL,
+  MTP_REQUIRE(page_size >= 1 && (page_size & (page_size - 1)) == 0 && max_pages <= 0x7fffffffll / page_size, MTP_EINVAL,
               "paged_plan: page_size=%lld (a power of two), %lld pages a row", (long long)page_size,
               (long long)max_pages);
   MTP_REQUIRE(tokens >= 0 && tokens <= 0x7fffffffll, MTP_EINVAL, "paged_plan: tokens=%lld", (long long)tokens);

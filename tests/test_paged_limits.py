@@ -94,3 +94,17 @@ def test_qk_norm_rope_of_the_most_tokens(gpu):
     # the same terms, added up in another order: 2^-11 for the result's rounding on either side and the fp32 sums' own
     for a, b in ((dqw, w1), (dkw, w2)):
         assert ((a.double() - b.double()).abs() <= 2 * 2.0 ** -11 * b.double().abs() * 1.01 + 1e-3).all()
+
+
+# --------------------------------------------------------------------------- sizes whose product passes 64 bits
+def test_products_of_sizes_do_not_wrap():
+    """page_size * max_pages and tokens * heads of 2^64: refused like every product past the limit (a wrapped one is 0)."""
+    from merak_amd import _lib
+    lib, A = _lib.lib(), 4096
+    plan = lambda pages, page: lib.mtp_paged_plan(*(A,) * 11, A + 64, A + 64, 2, pages, page, 8, 3, None)
+    attn = lambda T: lib.mtp_attn_paged(*(A,) * 8, lib.mtp_attn_paged_workspace_bytes(), T, 2, 8, 2, 128, 9, 16, 4, 1, 64, 0.1, 1,
+                                        None)
+    for pages, page in ((4, 2 ** 62), (2 ** 30, 2 ** 34), (2, 2 ** 62), (1, 2 ** 62), (2, 2 ** 30)):
+        assert plan(pages, page) == -1 and b"power of two" in lib.mtp_last_error(), (pages, page)
+    for T in (2 ** 61, 2 ** 62, 2 ** 27):
+        assert attn(T) == -1 and b"T=" in lib.mtp_last_error(), T
