@@ -121,7 +121,7 @@ struct Tiles {
     }
     const int upto = tok + (frac > 0 ? 1 : 0);
     const int end = e0 + (upto < n ? upto : n);
-    return end <= 0 ? 0 : (end + TK - 1) / TK;
+    return end <= 0 ? 0 : (end - 1) / TK + 1;      // end + TK - 1 may pass 2^31
   }
 };
 

@@ -108,3 +108,33 @@ def test_products_of_sizes_do_not_wrap():
         assert plan(pages, page) == -1 and b"power of two" in lib.mtp_last_error(), (pages, page)
     for T in (2 ** 61, 2 ** 62, 2 ** 27):
         assert attn(T) == -1 and b"T=" in lib.mtp_last_error(), T
+
+
+# --------------------------------------------------------------------------- lengths next to 2^31
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,new", [(torch.bfloat16, 1), (torch.float16, 5), (torch.bfloat16, 70)])
+def test_attn_paged_length_next_to_2_31(gpu, dtype, new):
+    """A table row of 2^27 - 1 pages of 16 tokens of which only the last is in the cache: 2^31 - 32 tokens read as zeros
+    (score 0, weight 1, value 0), 16 have scores about 22, with which their weights are of the size of that mass."""
+    page, d, rows = 16, 64, 2 ** 27 - 1
+    kv = page * rows
+    table = torch.full((1, rows), -1, dtype=torch.int32, device=gpu)
+    table[0, -1] = 0
+    k = torch.zeros(1, 1, page, d, dtype=dtype)
+    k[0, 0, :, 0] = 20 + torch.arange(page) * 0.125                       # exact in both types
+    v = torch.randn(1, 1, page, d, generator=gen(20)).to(dtype)
+    q = torch.zeros(new, 1, d, dtype=dtype)
+    q[:, :, 0] = 1.0
+    got = ops.attn_paged(q.to(gpu), k.to(gpu), v.to(gpu), table, torch.tensor([0, new], device=gpu),
+                         torch.tensor([kv], device=gpu), scale=1.0, max_new=new).double().cpu()[:, 0]
+    seen = torch.arange(kv - new + 1, kv + 1)                             # tokens of each row
+    real = (seen - (kv - page)).clamp_min(0)                              # of the last page
+    w = torch.exp(k[0, 0, :, 0].double()) * (torch.arange(page)[None] < real[:, None])
+    total = (seen - real).double()[:, None] + w.sum(1, keepdim=True)
+    ref, mag = w @ v[0, 0].double() / total, w @ v[0, 0].double().abs() / total
+    half = torch.finfo(dtype).eps / 2
+    # the 2^31 ones add up exactly in a lane (2^22 of them), and in fp32 over 2048 waves and their merges; the weights are
+    # rounded once each, the exponent's argument is off by 3 2^-24 of 23 log2(e)
+    bound = half * ref.abs() * 1.01 + torch.finfo(dtype).smallest_normal * half + (half + (2 * 2048 + 256) * U32) * 1.02 * mag
+    ratio = ((got - ref).abs() / bound.clamp_min(1e-30)).max()
+    assert not torch.isnan(got).any() and ratio <= 1, float(ratio)
