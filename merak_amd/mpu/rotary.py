@@ -21,7 +21,7 @@ class _QKNormRotary(torch.autograd.Function):
         ctx.save_for_backward(qkv, q_weight, k_weight, cos_table, sin_table, positions)
         ctx.n_q_heads, ctx.eps = n_q_heads, eps
         hd = cos_table.shape[1]
-        v = qkv.view(qkv.shape[0], -1, hd)[:, n_q_heads + k.shape[1]:]
+        v = qkv.view(qkv.shape[0], n_q_heads + 2 * k.shape[1], hd)[:, n_q_heads + k.shape[1]:]
         return q, k, v
 
     @staticmethod

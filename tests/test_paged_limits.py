@@ -138,3 +138,19 @@ def test_attn_paged_length_next_to_2_31(gpu, dtype, new):
     bound = half * ref.abs() * 1.01 + torch.finfo(dtype).smallest_normal * half + (half + (2 * 2048 + 256) * U32) * 1.02 * mag
     ratio = ((got - ref).abs() / bound.clamp_min(1e-30)).max()
     assert not torch.isnan(got).any() and ratio <= 1, float(ratio)
+
+
+# --------------------------------------------------------------------------- no tokens
+@pytest.mark.gpu
+@pytest.mark.parametrize("lead", [(0,), (0, 7), (3, 0)])
+def test_qk_norm_rotary_of_no_tokens(gpu, lead):
+    """An empty batch or sequence: empty heads, an empty gradient and weight gradients of zero."""
+    from merak_amd import mpu
+    d, hq, hk = 64, 4, 2
+    x = torch.zeros(*lead, (hq + 2 * hk) * d, dtype=torch.bfloat16, device=gpu, requires_grad=True)
+    w = [torch.ones(d, dtype=torch.bfloat16, device=gpu, requires_grad=True) for _ in range(2)]
+    table = torch.ones(5, d, device=gpu)
+    q, k, v = mpu.qk_norm_rotary(x, table, table, torch.zeros(lead, dtype=torch.int64, device=gpu), hq, *w)
+    assert q.shape == (*lead, hq, d) and k.shape == v.shape == (*lead, hk, d)
+    (q.sum() + k.sum() + v.sum()).backward()
+    assert x.grad.shape == x.shape and all(t.grad.shape == (d,) and not t.grad.any() for t in w)
