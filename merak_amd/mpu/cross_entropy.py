@@ -27,7 +27,7 @@ import torch
 
 from .. import ops
 from .initialize import get_model_parallel_rank, get_model_parallel_world_size
-from .utils import VocabUtility
+from .utils import VocabUtility, first_derivative_only
 
 
 def _vocab_range(partition_vocab_size):
@@ -65,6 +65,7 @@ class _VocabParallelCrossEntropy(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @first_derivative_only
     def backward(ctx, grad_output):
         logits, target_1d, row_max, row_sumexp = ctx.saved_tensors
         partition_vocab_size = logits.size()[-1]
@@ -102,6 +103,7 @@ class _VocabParallelCrossEntropyFused(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @first_derivative_only
     def backward(ctx, grad_output):
         (grad,) = ctx.saved_tensors
         grad_2d = grad.view(-1, grad.size()[-1])
@@ -222,6 +224,7 @@ class _LMHeadCrossEntropy(torch.autograd.Function):
         return losses.view(*target.shape)
 
     @staticmethod
+    @first_derivative_only
     def backward(ctx, grad_losses):
         dh, dw, db = ctx.saved_tensors
         g = grad_losses.reshape(-1)

@@ -21,7 +21,7 @@ from .initialize import get_model_parallel_rank, get_model_parallel_world_size
 from .mappings import (copy_to_model_parallel_region, gather_from_model_parallel_region,
                        reduce_from_model_parallel_region, scatter_to_model_parallel_region)
 from .random import get_rng_tracker
-from .utils import VocabUtility, divide
+from .utils import VocabUtility, divide, first_derivative_only
 
 _ACTIVATIONS = {None: None, "gelu_new": "gelu_new", "swiglu": "swiglu"}
 
@@ -105,6 +105,7 @@ class _LinearFunction(torch.autograd.Function):
         return y if activation is None else act
 
     @staticmethod
+    @first_derivative_only
     def backward(ctx, grad_out):
         x2d, weight, pre = ctx.saved_tensors
         g2d = grad_out.reshape(-1, grad_out.shape[-1])
@@ -137,6 +138,7 @@ class _EmbeddingFunction(torch.autograd.Function):
         return ops.embedding_gather(ids, weight, vocab_start, vocab_end)
 
     @staticmethod
+    @first_derivative_only
     def backward(ctx, grad_out):
         (ids,) = ctx.saved_tensors
         grad_out = grad_out if grad_out.dtype == ctx.wdtype else grad_out.to(ctx.wdtype)

@@ -10,6 +10,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import ops
+from .utils import first_derivative_only
 
 
 class _QKNormRotary(torch.autograd.Function):
@@ -25,6 +26,7 @@ class _QKNormRotary(torch.autograd.Function):
         return q, k, v
 
     @staticmethod
+    @first_derivative_only
     def backward(ctx, dq, dk, dv):
         qkv, q_weight, k_weight, cos_table, sin_table, positions = ctx.saved_tensors
         want_dw = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]

@@ -1,5 +1,7 @@
-"""Integer helpers of the model-parallel layers (Merak/core/mpu/utils.py:33-64,90-106)."""
+"""Helpers of the model-parallel layers (integers: Merak/core/mpu/utils.py:33-64,90-106)."""
 from __future__ import annotations
+
+import functools
 
 import torch
 
@@ -38,3 +40,32 @@ class VocabUtility:
     def vocab_range_from_global_vocab_size(global_vocab_size, rank, world_size):
         per_partition_vocab_size = divide(global_vocab_size, world_size)
         return VocabUtility.vocab_range_from_per_partition_vocab_size(per_partition_vocab_size, rank, world_size)
+
+
+class _NoFurtherDerivative(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, grad):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("second derivative of a function whose backward pass runs kernels autograd cannot look into")
+
+
+def first_derivative_only(backward):
+    """For the ``backward`` of an autograd function that calls kernels: with ``create_graph`` its results would look like
+    constants to autograd and the second derivative's terms through them would be left out; they raise instead.  (torch's
+    ``once_differentiable`` does so only where the incoming gradient has a graph, which that of a plain ``loss.sum()`` has
+    not.)"""
+
+    @functools.wraps(backward)
+    def wrapped(ctx, *grads):
+        if not torch.is_grad_enabled():      # the usual backward pass: nothing to add
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        mark = lambda t: None if t is None else _NoFurtherDerivative.apply(t.detach().requires_grad_(True))
+        return tuple(map(mark, out)) if isinstance(out, tuple) else mark(out)
+
+    return wrapped
