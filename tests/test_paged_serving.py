@@ -165,3 +165,59 @@ def test_verify_with_drafts_of_different_lengths(gpu):
     for bad in ([K + 1, 0, 0, 0], [0, 0, 0], [-2, 0, 0, 0]):
         with pytest.raises(ValueError, match="draft_lens"):
             dec.verify(last, drafts, u, draft_lens=bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", [0, 1])
+def test_speculative_steps_against_the_targets_own_logits(gpu, seed):
+    """top_k = 1 makes the target certain.  Every accepted draft and every drawn token is the argmax of the target's logits
+    at its position (from a decoder that got the text in one piece), every rejected draft is not; a request whose drafts
+    are those argmaxes has all of them accepted.  Positions whose two largest logits lie within the 2e-2 of the other
+    tests (norm-wise: of the root mean square of a row, on either side) are not judged."""
+    mc = model(gpu, 20 + seed)
+    m = on(gpu, mc)
+    g = gen(seed + 6)
+    prompt = torch.randint(0, V, (2, 17), generator=g)
+    dec = decoder(m, slots=2)
+    first = dec.step(prompt.reshape(-1).to(gpu), [17, 17]).cpu()
+    text = [prompt[r].tolist() + [int(first[r])] for r in range(2)]        # the last token is not in the cache yet
+    K, judged, all_kept = 4, 0, 0
+
+    def logits(seq):
+        return torch.nn.functional.linear(forward_fp32(mc, torch.tensor(seq)), mc[3].float())
+
+    def sure(row):
+        top = row.topk(2).values
+        return (top[0] - top[1]).item() > 2 * 2e-2 * row.square().mean().sqrt().item()
+
+    for _ in range(6):
+        greedy = list(text[0])                                            # the first request's drafts: its own argmaxes
+        clear = True
+        for _ in range(K):
+            row = logits(greedy)[-1]
+            clear &= sure(row)
+            greedy.append(int(row.argmax()))
+        clear &= sure(logits(greedy)[-1])
+        drafts = torch.stack([torch.tensor(greedy[-K:]), torch.randint(0, V, (K,), generator=g)])
+        if judged % 2:                                                    # the second request: one right draft, then noise
+            drafts[1, 0] = int(logits(text[1])[-1].argmax())
+        last = torch.tensor([t[-1] for t in text])
+        tokens, n = dec.verify(last.to(gpu), drafts.to(gpu), torch.rand(2, K + 1, generator=g).to(gpu), top_k=1)
+        tokens, n = tokens.cpu(), n.tolist()
+        if clear:
+            assert n[0] == K
+            all_kept += 1
+        for r in range(2):
+            rows = logits(text[r] + drafts[r].tolist())[len(text[r]) - 1:]   # of the last token, then behind each draft
+            for i in range(n[r]):
+                assert int(tokens[r, i]) == int(drafts[r, i])
+                assert not sure(rows[i]) or int(drafts[r, i]) == int(rows[i].argmax())
+            at = rows[n[r]]
+            if sure(at):
+                judged += 1
+                assert int(tokens[r, n[r]]) == int(at.argmax())
+                assert n[r] == K or int(drafts[r, n[r]]) != int(at.argmax())
+            assert (tokens[r, n[r] + 1:] == -1).all()
+            text[r] += tokens[r, :n[r] + 1].tolist()
+            assert dec.lens[r].item() == len(text[r]) - 1
+    assert judged >= 8 and all_kept >= 3, (judged, all_kept)
