@@ -948,6 +948,7 @@ def attn_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
         raise ValueError("attn_paged: out must be a contiguous, 16-byte aligned tensor like q")
     if workspace is None:
         workspace = attn_paged_workspace(dev)
+    _own("attn_paged", "workspace", workspace)
     with _device(dev):
         _lib.check(_lib.lib().mtp_attn_paged(_p(q), _p(k_cache), _p(v_cache), _p(block_tables), _p(cu), _p(kv_lens), _p(out),
                                              _p(workspace), workspace.numel() * workspace.element_size(), T, R, n_q, n_kv,

@@ -154,3 +154,16 @@ def test_qk_norm_rotary_of_no_tokens(gpu, lead):
     assert q.shape == (*lead, hq, d) and k.shape == v.shape == (*lead, hk, d)
     (q.sum() + k.sum() + v.sum()).backward()
     assert x.grad.shape == x.shape and all(t.grad.shape == (d,) and not t.grad.any() for t in w)
+
+
+# --------------------------------------------------------------------------- memory that a call writes
+@pytest.mark.gpu
+def test_attn_paged_refuses_a_strided_workspace(gpu):
+    """Every second byte of a buffer: as many elements as the call needs, but the bytes between are not its own."""
+    need = ops.attn_paged_workspace(gpu).numel()
+    k = torch.zeros(1, 1, 16, 64, dtype=torch.bfloat16, device=gpu)
+    args = (torch.zeros(1, 1, 64, dtype=torch.bfloat16, device=gpu), k, k, torch.zeros(1, 1, dtype=torch.int32, device=gpu),
+            torch.tensor([0, 1], device=gpu), torch.tensor([3], device=gpu))
+    with pytest.raises(ValueError, match="workspace"):
+        ops.attn_paged(*args, workspace=torch.zeros(2 * need, dtype=torch.uint8, device=gpu)[::2])
+    ops.attn_paged(*args, workspace=torch.zeros(need + 64, dtype=torch.uint8, device=gpu)[64:])
