@@ -28,19 +28,20 @@
 // merges them in order, so the result does not depend on which one that is.
 //
 // Two kernels, chosen by the most rows a tile can have:
-//   narrow  up to 32 RB rows (RB = 1, 2), bound by HBM: the waves of a workgroup take turns with the units of its run,
-//           each with a ring of LDS slots of its own and no barrier in the loop, and are merged at the end;
+//   narrow  up to 32 rows, bound by HBM: the waves of a workgroup take turns with the units of its run, each with a ring
+//           of LDS slots of its own and no barrier in the loop, and are merged at the end;
 //   wide    256 rows, 32 per wave, bound by the matrix cores: the waves share each unit's keys and values.
 #include "gemm_bf16_kernel.h"
 
 namespace {
 
 constexpr int AP_PAGE_MIN = 16;      // tokens per DMA block
-// a tile's start (first keys under way, queries, merge, output) in units
+// A tile's start (first keys under way, queries, merge, output) in units, as runs are dealt.  Narrow with 2, 8 and 16:
+// decode of 64 requests 110, 100 and 102 us, drafts of 32 requests 68, 65 and 66.  Wide with 1, 4 and 12: prompts of 4
+// requests 675, 636 and 660 us, 24 tokens of 32 requests 91, 84 and 88.
 constexpr int AP_START_NARROW = 8;
 constexpr int AP_START_WIDE = 4;
-constexpr int AP_MAX_WGS = 1024;     // arrival counters: 4 bytes each at the head of the workspace
-constexpr int64_t AP_COUNTER_BYTES = 4096;
+constexpr int64_t AP_COUNTER_BYTES = 4096;     // arrival counters: 4 bytes a workgroup at the head of the workspace
 
 struct PagedArgs {
   const uint16_t* q;         // [T, n_q, D]
@@ -218,7 +219,7 @@ __device__ __forceinline__ float half_max(float v) {
 // place of element d of a row in the merge area
 template <int D> __device__ __forceinline__ int merge_at(int row, int d) { return row * D + (d ^ ((row & 7) << 2)); }
 
-template <int D, bool F16, int RB, int NB>
+template <int D, bool F16, int NB>
 struct Wave {
   using X = X16<F16>;
   static constexpr int KS = D / 16, DT = D / 32, ROW = D * 2;
@@ -229,41 +230,38 @@ struct Wave {
   // LAZY + SHIFT = 15 stays below the largest half, 2^16: the maximum may lag behind by LAZY binary orders.  Times of f16
   // decode of 64 requests and of prompts: 102 and 665 us, with LAZY 8 and SHIFT 7 102 and 669, with 2 and 13 101 and 666.
   static constexpr float LAZY = F16 ? 4.0f : 8.0f, SHIFT = F16 ? 11.0f : 0.0f;
-  bf16x8_t qf[RB][KS];
-  f32x16_t o[RB][DT];
-  float m[RB], l[RB];
-  int lim[RB];               // first token the lane's row does not see
-  u32x4_t pf[RB][2 * NB];    // probabilities of the unit, as the second product's operand
+  bf16x8_t qf[KS];
+  f32x16_t o[DT];
+  float m, l;
+  int lim;                   // first token the lane's row does not see
+  u32x4_t pf[2 * NB];        // probabilities of the unit, as the second product's operand
 
-  // rows row0 + 32 rb + lane % 32 of the tile, of which `rows` exist
+  // rows row0 + lane % 32 of the tile, of which `rows` exist
   __device__ __forceinline__ void start(const PagedArgs& p, const Request& q, int kvh, int row0, int rows) {
     const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    int row = row0 + c;
+    if (row >= rows) row = rows - 1;          // a copy of the last row, never stored
+    const int tok = row / p.group, g = row - tok * p.group;
+    const uint16_t* src = p.q + ((int64_t)(q.t0 + tok) * p.n_q + kvh * p.group + g) * D + 8 * h;
 #pragma unroll
-    for (int rb = 0; rb < RB; rb++) {
-      int row = row0 + 32 * rb + c;
-      if (row >= rows) row = rows - 1;        // a copy of the last row, never stored
-      const int tok = row / p.group, g = row - tok * p.group;
-      const uint16_t* src = p.q + ((int64_t)(q.t0 + tok) * p.n_q + kvh * p.group + g) * D + 8 * h;
+    for (int s = 0; s < KS; s++) qf[s] = *reinterpret_cast<const bf16x8_t*>(src + 16 * s);
+    // the queries are waited for here, once: left to their first use, the wait would sit in the loop and drain the
+    // DMA in flight at every step
 #pragma unroll
-      for (int s = 0; s < KS; s++) qf[rb][s] = *reinterpret_cast<const bf16x8_t*>(src + 16 * s);
-      // the queries are waited for here, once: left to their first use, the wait would sit in the loop and drain the
-      // DMA in flight at every step
+    for (int s = 0; s < KS; s++) asm volatile("" : "+v"(qf[s]));
+    lim = q.kv - q.n + tok + 1;
+    m = -INFINITY;
+    l = 0.0f;
 #pragma unroll
-      for (int s = 0; s < KS; s++) asm volatile("" : "+v"(qf[rb][s]));
-      lim[rb] = q.kv - q.n + tok + 1;
-      m[rb] = -INFINITY;
-      l[rb] = 0.0f;
+    for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-      for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[rb][dt][i] = 0.0f;
-    }
+      for (int i = 0; i < 16; i++) o[dt][i] = 0.0f;
   }
 
   // scores of the unit's keys (LDS tile `ks`, first token tok0), running maximum and sum, probabilities
   template <bool MASK> __device__ __forceinline__ void scores(const char* ks, int tok0, float c) {
     const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
-    f32x16_t s[RB][NB];
+    f32x16_t s[NB];
     bf16x8_t a[KS][NB];
 #pragma unroll
     for (int k = 0; k < KS; k++)
@@ -273,63 +271,57 @@ struct Wave {
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
-      for (int rb = 0; rb < RB; rb++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) s[rb][b][i] = 0.0f;
+      for (int i = 0; i < 16; i++) s[b][i] = 0.0f;
 #pragma unroll
     for (int k = 0; k < KS; k++)
 #pragma unroll
       for (int b = 0; b < NB; b++)        // neighbouring products add to different blocks: none waits for the one before
-#pragma unroll
-        for (int rb = 0; rb < RB; rb++) s[rb][b] = X::mfma32(a[k][b], qf[rb][k], s[rb][b]);
+        s[b] = X::mfma32(a[k][b], qf[k], s[b]);
     // fragments are read KS products ahead
     __builtin_amdgcn_sched_group_barrier(SG_DS_RD, KS, 0);
 #pragma unroll
     for (int i = 0; i < (NB - 1) * KS; i++) {
-      __builtin_amdgcn_sched_group_barrier(SG_MFMA, RB, 0);
+      __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
       __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 1, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(SG_MFMA, KS * RB, 0);
-#pragma unroll
-    for (int rb = 0; rb < RB; rb++) {
-      if (MASK) {
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-          for (int i = 0; i < 16; i++)
-            if (tok0 + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) >= lim[rb]) s[rb][b][i] = -INFINITY;
-      }
-      float mx = s[rb][0][0];
+    __builtin_amdgcn_sched_group_barrier(SG_MFMA, KS, 0);
+    if (MASK) {
 #pragma unroll
       for (int b = 0; b < NB; b++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[rb][b][i]);
-      mx = half_max(mx);
-      // The maximum only has to keep the exponentials in range: it is moved (and O and l rescaled) when a row's has
-      // grown by more than LAZY binary orders, not at every step.  A row that has seen nothing yet stays at -inf.
-      if (__any((mx - m[rb]) * c > LAZY)) {
-        const float mn = fmaxf(m[rb], mx);
-        const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m[rb] - mn) * c);
-        m[rb] = mn;
-        l[rb] *= f;
+        for (int i = 0; i < 16; i++)
+          if (tok0 + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) >= lim) s[b][i] = -INFINITY;
+    }
+    float mx = s[0][0];
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++)
+    for (int b = 0; b < NB; b++)
 #pragma unroll
-          for (int i = 0; i < 16; i++) o[rb][dt][i] *= f;
-      }
-      const float mc = SHIFT - (m[rb] == -INFINITY ? 0.0f : m[rb] * c);
-      // the sum takes the probabilities as the second product sees them, rounded: half as many instructions (a dot
-      // product with ones adds two), and numerator and denominator then share each rounding
+      for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[b][i]);
+    mx = half_max(mx);
+    // The maximum only has to keep the exponentials in range: it is moved (and O and l rescaled) when a row's has
+    // grown by more than LAZY binary orders, not at every step.  A row that has seen nothing yet stays at -inf.
+    if (__any((mx - m) * c > LAZY)) {
+      const float mn = fmaxf(m, mx);
+      const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
+      m = mn;
+      l *= f;
 #pragma unroll
-      for (int b = 0; b < NB; b++) {
+      for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[rb][b][i] = __builtin_amdgcn_exp2f(fmaf(s[rb][b][i], c, mc));
+        for (int i = 0; i < 16; i++) o[dt][i] *= f;
+    }
+    const float mc = SHIFT - (m == -INFINITY ? 0.0f : m * c);
+    // the sum takes the probabilities as the second product sees them, rounded: half as many instructions (a dot
+    // product with ones adds two), and numerator and denominator then share each rounding
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
+    for (int b = 0; b < NB; b++) {
 #pragma unroll
-          for (int e = 0; e < 4; e++) pf[rb][2 * b + k][e] = X::pack2(s[rb][b][8 * k + 2 * e], s[rb][b][8 * k + 2 * e + 1]);
-          l[rb] = X::sum8(__builtin_bit_cast(bf16x8_t, pf[rb][2 * b + k]), l[rb]);
-        }
+      for (int i = 0; i < 16; i++) s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, mc));
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) pf[2 * b + k][e] = X::pack2(s[b][8 * k + 2 * e], s[b][8 * k + 2 * e + 1]);
+        l = X::sum8(__builtin_bit_cast(bf16x8_t, pf[2 * b + k]), l);
       }
     }
   }
@@ -354,37 +346,34 @@ struct Wave {
 #pragma unroll
     for (int k = 0; k < 2 * NB; k++)
 #pragma unroll
-      for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-        for (int rb = 0; rb < RB; rb++) o[rb][dt] = X::mfma32(vf[k][dt], __builtin_bit_cast(bf16x8_t, pf[rb][k]), o[rb][dt]);
+      for (int dt = 0; dt < DT; dt++) o[dt] = X::mfma32(vf[k][dt], __builtin_bit_cast(bf16x8_t, pf[k]), o[dt]);
     // 16 tokens' fragments are read while the previous ones' are multiplied
     __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 2 * DT, 1);
 #pragma unroll
     for (int i = 0; i < (2 * NB - 1) * DT; i++) {
-      __builtin_amdgcn_sched_group_barrier(SG_MFMA, RB, 1);
+      __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 1);
       __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 2, 1);
     }
-    __builtin_amdgcn_sched_group_barrier(SG_MFMA, DT * RB, 1);
+    __builtin_amdgcn_sched_group_barrier(SG_MFMA, DT, 1);
   }
 
   // four consecutive dims of the lane's row: 32 dt + 8 i + 4 h
-  __device__ __forceinline__ f32x4_t quad(int rb, int dt, int i) const {
-    return f32x4_t{o[rb][dt][4 * i], o[rb][dt][4 * i + 1], o[rb][dt][4 * i + 2], o[rb][dt][4 * i + 3]};
+  __device__ __forceinline__ f32x4_t quad(int dt, int i) const {
+    return f32x4_t{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
   }
 
-  // row block rb as fp32 [32][D] and (m, l) per row; groups of four floats are swizzled by the row (merge_at), so that
-  // the lanes' rows fall into different banks
-  __device__ __forceinline__ void to_lds(int rb, float* dst, float* ml) const {
+  // the rows as fp32 [32][D] and (m, l) per row; groups of four floats are swizzled by the row (merge_at), so that the
+  // lanes' rows fall into different banks
+  __device__ __forceinline__ void to_lds(float* dst, float* ml) const {
     const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        *reinterpret_cast<f32x4_t*>(dst + merge_at<D>(row, 32 * dt + 8 * i + 4 * h)) =
-            quad(rb, dt, i);
-    const float sum = l[rb] + __shfl_xor(l[rb], 32, 64);
+        *reinterpret_cast<f32x4_t*>(dst + merge_at<D>(row, 32 * dt + 8 * i + 4 * h)) = quad(dt, i);
+    const float sum = l + __shfl_xor(l, 32, 64);
     if (h == 0) {
-      ml[2 * row] = m[rb];
+      ml[2 * row] = m;
       ml[2 * row + 1] = sum;
     }
   }
@@ -507,11 +496,12 @@ __device__ __forceinline__ void merge_if_last(const PagedArgs& p, const Request&
 }
 
 // ---- narrow tiles: the waves take turns with the units ------------------------------------------------------
-template <int D, bool F16, int RB, int WAVES, int RING>
-__global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const PagedArgs p) {
-  constexpr int TK = 32, BM = 32 * RB, THREADS = WAVES * 64;
-  constexpr int ITEM = TK * D * 2, DMAS = ITEM / 1024, AHEAD = RING - 1;
-  static_assert(32 * D * 4 <= RING * ITEM && AHEAD * DMAS < 64, "merge area / vmcnt range");
+template <int D, bool F16>
+__global__ __launch_bounds__(512) void attn_paged_narrow_kernel(const PagedArgs p) {
+  constexpr int WAVES = 8, RING = 2;                     // keys or values of one unit a slot
+  constexpr int TK = 32, BM = 32, THREADS = WAVES * 64;
+  constexpr int ITEM = TK * D * 2, DMAS = ITEM / 1024;
+  static_assert(BM * D * 4 <= RING * ITEM, "merge area");
   __shared__ __attribute__((aligned(1024))) char lds[WAVES * RING * ITEM];
   __shared__ float ml[WAVES][64];
   const int tid = threadIdx.x;
@@ -568,7 +558,7 @@ __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const Pag
 
         // ---- this wave's units of [ua, ub) ----
         const int n_my = ub - ua > wave ? (ub - ua - wave + WAVES - 1) / WAVES : 0, n_items = 2 * n_my;
-        Wave<D, F16, RB, 1> st;
+        Wave<D, F16, 1> st;
         st.start(p, q, kvh, j * BM, all);
         int pg[2];
         auto fetch_pages = [&](int i) {
@@ -588,57 +578,48 @@ __global__ __launch_bounds__(WAVES * 64) void attn_paged_narrow_kernel(const Pag
           }
           if ((it & 1) && it + 1 < n_items) fetch_pages((it + 1) >> 1);
         };
-        auto wait_item = [&](int it) {
-          const int after = n_items - 1 - it;
-          if (after >= AHEAD) wait_vm_at_most<AHEAD * DMAS>();
-          else if (AHEAD > 2 && after == 2) wait_vm_at_most<2 * DMAS>();
-          else if (AHEAD > 1 && after == 1) wait_vm_at_most<DMAS>();
+        auto wait_item = [&](int it) {        // one item may be under way behind it
+          if (it + 1 < n_items) wait_vm_at_most<DMAS>();
           else wait_vm_at_most<0>();
         };
-        static_assert(AHEAD <= 3, "wait_item");
-        if (n_my > 0) fetch_pages(0);
-#pragma unroll
-        for (int it = 0; it < AHEAD; it++)
-          if (it < n_items) issue(it);
+        if (n_my > 0) {
+          fetch_pages(0);
+          issue(0);
+        }
         for (int i = 0; i < n_my; i++) {
           const int tok = (ua + wave + WAVES * i) * TK;
-          if (2 * i + AHEAD < n_items) issue(2 * i + AHEAD);
+          issue(2 * i + 1);
           wait_item(2 * i);
           // always with the mask: it hides behind the memory, and a second path without it made the compiler copy the
           // accumulators where the two meet (decode of 64 requests 98 -> 114 us)
-          st.template scores<true>(ring + ((2 * i) % RING) * ITEM, tok, p.scale_log2e);
-          if (2 * i + 1 + AHEAD < n_items) issue(2 * i + 1 + AHEAD);
+          st.template scores<true>(ring, tok, p.scale_log2e);
+          if (2 * i + 2 < n_items) issue(2 * i + 2);
           wait_item(2 * i + 1);
-          st.values(ring + ((2 * i + 1) % RING) * ITEM);
+          st.values(ring + ITEM);
         }
 
-        // ---- the waves' results, a row block at a time ----
+        // ---- the waves' results ----
+        __syncthreads();                      // all units read
+        st.to_lds(reinterpret_cast<float*>(lds + wave * (RING * ITEM)), ml[wave]);
+        __syncthreads();
+        for (int idx = tid; idx < rows * (D / 4); idx += THREADS) {
+          const int row = idx / (D / 4), d = idx % (D / 4) * 4;
+          float mstar = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int rb = 0; rb < RB; rb++) {
-          if (32 * rb >= rows) break;
-          __syncthreads();                    // all units read / the previous block taken
-          st.to_lds(rb, reinterpret_cast<float*>(lds + wave * (RING * ITEM)), ml[wave]);
-          __syncthreads();
-          const int here = rows - 32 * rb < 32 ? rows - 32 * rb : 32;
-          for (int idx = tid; idx < here * (D / 4); idx += THREADS) {
-            const int row = idx / (D / 4), d = idx % (D / 4) * 4;
-            float mstar = -INFINITY, sum = 0.0f;
+          for (int i = 0; i < WAVES; i++) mstar = fmaxf(mstar, ml[i][2 * row]);
+          f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < WAVES; i++) mstar = fmaxf(mstar, ml[i][2 * row]);
-            f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < WAVES; i++) {
-              const float f = part_scale(ml[i][2 * row], mstar, p.scale_log2e);
-              acc += *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(lds + i * (RING * ITEM)) + merge_at<D>(row, d)) * f;
-              sum += ml[i][2 * row + 1] * f;
-            }
-            if (first == last) {
-              store_out<F16>(out_row<D>(p, q, kvh, j * BM + 32 * rb + row) + d, acc, inverse(sum));
-            } else {
-              const int dst = slot_of(w, first) * STRIDE;
-              part.store4(dst + (32 * rb + row) * D + d, acc);
-              if (d == 0) part.store2(dst + BM * D + 2 * (32 * rb + row), mstar, sum);
-            }
+          for (int i = 0; i < WAVES; i++) {
+            const float f = part_scale(ml[i][2 * row], mstar, p.scale_log2e);
+            acc += *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(lds + i * (RING * ITEM)) + merge_at<D>(row, d)) * f;
+            sum += ml[i][2 * row + 1] * f;
+          }
+          if (first == last) {
+            store_out<F16>(out_row<D>(p, q, kvh, j * BM + row) + d, acc, inverse(sum));
+          } else {
+            const int dst = slot_of(w, first) * STRIDE;
+            part.store4(dst + row * D + d, acc);
+            if (d == 0) part.store2(dst + BM * D + 2 * row, mstar, sum);
           }
         }
         if (first != last) merge_if_last<D, F16, BM, THREADS>(p, q, kvh, j, rows, first, last);
@@ -709,7 +690,7 @@ __global__ __launch_bounds__(512, 2) void attn_paged_wide_kernel(const PagedArgs
 
         const int row0 = 32 * wave;
         const bool active = row0 < rows;
-        Wave<D, F16, 1, 2> st;
+        Wave<D, F16, 2> st;
         st.start(p, q, kvh, j * BM + row0, all);
         const int lim0 = q.kv - q.n + (j * BM + row0) / p.group + 1;   // what the wave's first row sees
         int page = page_at(p, r, q.kv, ua * TK + (wave & 3) * AP_PAGE_MIN);
@@ -757,13 +738,13 @@ __global__ __launch_bounds__(512, 2) void attn_paged_wide_kernel(const PagedArgs
 
         if (first == last) {
           const int lane = tid & 63, c = lane & 31, h = lane >> 5;
-          const float inv = inverse(st.l[0] + __shfl_xor(st.l[0], 32, 64));
+          const float inv = inverse(st.l + __shfl_xor(st.l, 32, 64));
           if (row0 + c < rows) {
             uint16_t* dst = out_row<D>(p, q, kvh, j * BM + row0 + c);
 #pragma unroll
             for (int dt = 0; dt < D / 32; dt++)
 #pragma unroll
-              for (int i = 0; i < 4; i++) store_out<F16>(dst + 32 * dt + 8 * i + 4 * h, st.quad(0, dt, i), inv);
+              for (int i = 0; i < 4; i++) store_out<F16>(dst + 32 * dt + 8 * i + 4 * h, st.quad(dt, i), inv);
           }
         } else {
           // through LDS, 32 dims at a time in the wave's own quarter, for stores of whole lines
@@ -774,7 +755,7 @@ __global__ __launch_bounds__(512, 2) void attn_paged_wide_kernel(const PagedArgs
           for (int dt = 0; dt < D / 32; dt++) {
             wave_lds_sync();
 #pragma unroll
-            for (int i = 0; i < 4; i++) *reinterpret_cast<f32x4_t*>(mine + c * 36 + 8 * i + 4 * h) = st.quad(0, dt, i);
+            for (int i = 0; i < 4; i++) *reinterpret_cast<f32x4_t*>(mine + c * 36 + 8 * i + 4 * h) = st.quad(dt, i);
             wave_lds_sync();
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -783,8 +764,8 @@ __global__ __launch_bounds__(512, 2) void attn_paged_wide_kernel(const PagedArgs
                 part.store4(dst + (row0 + row) * D + 32 * dt + d, *reinterpret_cast<const f32x4_t*>(mine + row * 36 + d));
             }
           }
-          const float sum = st.l[0] + __shfl_xor(st.l[0], 32, 64);
-          if (lane < 32 && row0 + lane < rows) part.store2(dst + BM * D + 2 * (row0 + lane), st.m[0], sum);
+          const float sum = st.l + __shfl_xor(st.l, 32, 64);
+          if (lane < 32 && row0 + lane < rows) part.store2(dst + BM * D + 2 * (row0 + lane), st.m, sum);
           merge_if_last<D, F16, BM, THREADS>(p, q, kvh, j, rows, first, last);
         }
         __syncthreads();
@@ -796,18 +777,23 @@ __global__ __launch_bounds__(512, 2) void attn_paged_wide_kernel(const PagedArgs
 
 constexpr int NARROW_WGS = 256;      // one per CU: 128 KiB of LDS each
 constexpr int WIDE_WGS = 256;        // one per CU: 128 KiB
+static_assert(NARROW_WGS * 4 <= AP_COUNTER_BYTES && WIDE_WGS * 4 <= AP_COUNTER_BYTES, "arrival counters");
 
+// Narrow up to 32 rows a tile: 64 requests of up to 8000 tokens, one token each, 32 + 8 heads: 85 us (wide: 98), 8 tokens
+// each 66 (71); one request of 130001 tokens 95 (112), its 8 tokens 100 (113); 12 + 12 heads of 64, 24 tokens 39 (49).
+// From 33 rows on wide; a narrow form with two row blocks and four waves was slower nearly everywhere: 9 tokens of 64
+// requests 82 (wide: 77), 16 tokens of 4 requests 30 (20), 5 tokens of 96 requests with 64 + 8 heads 81 (71); only one
+// request of 130001 tokens gained, 9 tokens 111 (116).
+// min_units, the shortest run: few requests then keep to few workgroups.  Narrow with 2, 8 and 32 units: four requests of
+// up to 900 tokens 12.2, 12.5 and 21.5 us; wide with 1, 4 and 16: a prompt of 300 tokens 33.5, 35.7 and 51 us, one of 1500
+// 60.6, 60.4 and 65.3; the long cases do not depend on it.
 template <int D, bool F16>
 void launch(const PagedArgs& base, int rows, hipStream_t s) {
   PagedArgs a = base;
   if (rows <= 32) {
     a.wgs = NARROW_WGS;
     a.min_units = 8;
-    hipLaunchKernelGGL((attn_paged_narrow_kernel<D, F16, 1, 8, 2>), dim3(a.wgs), dim3(512), 0, s, a);
-  } else if (rows <= 64) {
-    a.wgs = NARROW_WGS;
-    a.min_units = 8;
-    hipLaunchKernelGGL((attn_paged_narrow_kernel<D, F16, 2, 4, 4>), dim3(a.wgs), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((attn_paged_narrow_kernel<D, F16>), dim3(a.wgs), dim3(512), 0, s, a);
   } else {
     a.wgs = WIDE_WGS;
     a.min_units = 4;
