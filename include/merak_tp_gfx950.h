@@ -536,8 +536,8 @@ int mtp_qk_norm_rope_bwd(const void* dq, const void* dk, const void* dv, const v
 /* The serving form: queries to q_out, keys (normed and rotated) and values
  * (copied) to slots[t] of k_cache and v_cache [n_pages, n_kv_heads, page_size,
  * head_dim].  A row whose slot is outside the cache, or whose position is
- * outside the tables, appends nothing.  Two rows with one slot: one of them
- * stays, which is not said.  bf16 or f16; page_size a power of two. */
+ * outside the tables, appends nothing.  Two rows with one slot (mtp_paged_plan
+ * gives none): each 16 bytes there are one row's or the other's.  bf16 or f16; page_size a power of two. */
 int mtp_qk_norm_rope_append(const void* qkv, const void* cos_table, const void* sin_table, int table_dtype,
                             const int64_t* positions, const int64_t* slots,
                             const void* q_weight, const void* k_weight,
@@ -560,9 +560,11 @@ int mtp_qk_norm_rope_append(const void* qkv, const void* cos_table, const void* 
  * outside the cache read as zeros.  What lies in a page behind a request's
  * length is not read into the result, whatever it holds; keys and values below
  * it are expected to be finite.
- * max_new bounds the new tokens of a request and len_bound kv_lens, both known
- * on the host; they choose how work is laid out, and a request that passes
- * max_new is still computed.  workspace:
+ * max_new, known on the host, bounds the new tokens of a request and chooses
+ * between the two kernels (rows of a tile up to 32, or more); a request that
+ * passes it is still computed.  len_bound, the bound of kv_lens that
+ * mtp_attn_decode wants too, must not be negative and has no effect: the work is
+ * laid out from the lengths on the device.  workspace:
  * mtp_attn_paged_workspace_bytes() bytes for any shape, 16-byte aligned; ITS
  * FIRST 4096 BYTES MUST BE ZERO before the first launch that uses it and are
  * zero again after each.  Launches that share a workspace must not overlap.

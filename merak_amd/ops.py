@@ -892,7 +892,8 @@ def qk_norm_rope_append(qkv: torch.Tensor, cos_table: torch.Tensor, sin_table: t
                         q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
                         eps: float = 1e-6) -> torch.Tensor:
     """``qk_norm_rope`` for serving: returns q [T, n_q, head_dim] and writes the keys and the values of each row to
-    ``slots[t]`` of the caches [n_pages, n_kv, page_size, head_dim] (-1: nowhere)."""
+    ``slots[t]`` of the caches [n_pages, n_kv, page_size, head_dim] (-1: nowhere; no slot twice, or parts of either row
+    stay)."""
     dev = _require_gpu(qkv, cos_table, sin_table, positions, slots, k_cache, v_cache, q_weight, k_weight)
     n_pages, n_kv, page_size, hd = _pages("qk_norm_rope_append", k_cache, v_cache)
     if cos_table.dim() != 2 or cos_table.shape[1] != hd or k_cache.dtype != qkv.dtype or v_cache.dtype != qkv.dtype:
@@ -923,8 +924,9 @@ def attn_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal grouped-query attention of each request's new tokens over its pages, any mix of single tokens, drafts and
     prompts.  q [T, n_q, head_dim]; rows cu[r] .. cu[r+1]-1 are request r's, whose last one is token kv_lens[r] - 1 of
-    the pages that row r of ``block_tables`` names.  ``max_new`` / ``len_bound``: upper bounds of a request's new tokens
-    and of kv_lens known on the host (they choose how the work is laid out).  Rows of no request are left as they were in
+    the pages that row r of ``block_tables`` names.  ``max_new``: upper bound of a request's new tokens known on the host
+    (it chooses the kernel; a request that passes it is still computed).  ``len_bound`` is taken as by ``attn_decode`` and
+    has no effect: the work is laid out from the lengths on the device.  Rows of no request are left as they were in
     ``out`` (unspecified in a new tensor).  ``workspace``: from ``attn_paged_workspace``."""
     dev = _require_gpu(q, k_cache, v_cache, block_tables, cu, kv_lens, workspace, out)
     n_pages, n_kv, page_size, hd = _pages("attn_paged", k_cache, v_cache)
