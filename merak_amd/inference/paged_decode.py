@@ -26,9 +26,9 @@ class PagedLlamaDecoder:
 
     ``append(tokens, new_lens)`` adds ``new_lens[r]`` tokens to request r (host numbers; the tokens of all requests one
     after the other) and returns the final-norm output of every new token.  A request that finds no page, or whose length
-    would pass ``max_len``, is refused: ``self.granted[r]`` is False, its rows are meaningless and its state is as before.  ``release([r, ...])`` gives requests'
-    pages back.  ``q_norms`` / ``k_norms``: norm weights [head_dim] of each block's query and key heads, for models that
-    have them."""
+    would pass ``max_len``, is refused: ``self.granted[r]`` is False, its rows are meaningless and its state is as before.
+    ``release([r, ...])`` gives requests' pages back.  ``q_norms`` / ``k_norms``: norm weights [head_dim] of each block's
+    query and key heads, for models that have them."""
 
     def __init__(self, embed: torch.Tensor, blocks: List[LlamaBlockWeights], final_norm: torch.Tensor,
                  lm_head: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim: int = 128, eps: float = 1e-5,
