@@ -31,6 +31,10 @@
 //   narrow  up to 32 rows, bound by HBM: the waves of a workgroup take turns with the units of its run, each with a ring
 //           of LDS slots of its own and no barrier in the loop, and are merged at the end;
 //   wide    256 rows, 32 per wave, bound by the matrix cores: the waves share each unit's keys and values.
+// With 32 + 8 heads of 128: decode of 64 requests of 200 to 8192 tokens 95 us for 575 MB (6.0 TB/s; read-only streams
+// reach 7.0), one token of a request of 130001 88 us (6.0 TB/s), five tokens of 32 requests 60 us (5.0 TB/s), prompts of
+// 1900 to 4100 tokens behind up to 5000 562 us for 556 GFLOP (0.99 PFLOP/s; large products reach 1.43): the waves of a
+// workgroup meet at a barrier every 64 tokens, so the two of a SIMD multiply and exponentiate at the same time.
 #include "gemm_bf16_kernel.h"
 
 namespace {

@@ -15,7 +15,10 @@
 // a head and the 8 matching ones of the second half, so both halves of a rotation sit in one lane (no exchange) and
 // the mean is three or two butterfly steps over the D / 16 lanes of a head.  One wave walks the heads of one token, so
 // the table row is loaded once per token and stays in registers; with few tokens the heads of a token are dealt to
-// several waves.
+// several waves.  8192 tokens of 32 + 8 heads of 128 in bf16: forward 36 us for 176 MB (5.0 TB/s; a copy of 168 MB runs
+// at 5.0 to 5.8), backward 70 us for 294 MB (4.2 TB/s: 200 registers a lane, two waves per SIMD, do not keep enough loads
+// under way) and 4.6 us for the weight gradients' sum.  Append of 8191 tokens of 8 + 1 heads 12 us for 50 MB, of 32
+// tokens 3.6 us: the launch.
 #include "mtp_common.h"
 
 namespace {
