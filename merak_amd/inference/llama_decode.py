@@ -133,6 +133,8 @@ def hf_weights(model, max_len: int, head_norms: bool = False):
     if getattr(model.lm_head, "bias", None) is not None:
         refuse("lm_head has a bias")
     rp = getattr(cfg, "rope_parameters", None) or getattr(cfg, "rope_scaling", None) or {}
+    if any(isinstance(v, dict) for v in rp.values()):
+        refuse("rotary parameters by kind of layer")
     if rp.get("partial_rotary_factor", 1.0) != 1.0:
         refuse(f"partial_rotary_factor {rp['partial_rotary_factor']}")
     theta = rp.get("rope_theta", getattr(cfg, "rope_theta", 10000.0))

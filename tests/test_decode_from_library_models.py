@@ -88,6 +88,8 @@ def test_other_arithmetic_is_refused():
     refused("Granite", "scores scaled|multiplier|scaling", attention_multiplier=0.5)
     refused("Granite", "residual_multiplier", residual_multiplier=0.3)
     refused("Mistral", "sliding window", sliding_window=32)
+    by_kind = {"full_attention": {"rope_theta": 5e5, "rope_type": "default"}}
+    refused("Llama", "by kind of layer", change=lambda m: m.config.__dict__.update(rope_parameters=by_kind))
     refused("Qwen3", "sliding window", use_sliding_window=True, sliding_window=32, max_window_layers=1)
 
 
