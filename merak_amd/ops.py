@@ -50,8 +50,16 @@ def _require_gpu(*ts: torch.Tensor) -> torch.device:
     return dev
 
 
+def _public_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the handle without the Stream object around it: 1.8 us of a small launch; a torch without this name has the other way
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _public_stream)
+
+
 def _stream(dev: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(dev.index)   # without the Stream object around it: 1.8 us of a small launch
+    return _raw_stream(dev.index)
 
 
 class _Here:

@@ -200,3 +200,16 @@ def test_decoder_with_many_slots(gpu):
         assert rel(out[i:i + 1], forward_fp32(mc, text[r, :lens[r] + 1])[-1:]) < 2e-2
     dec.append(text[1, :2].to(gpu), [0, 2] + [0] * (S - 2))               # no page left
     assert not dec.granted[1] and dec.granted.sum() == S - 1
+
+
+def test_both_ways_to_the_current_stream_agree(gpu, monkeypatch):
+    side = torch.cuda.Stream(gpu)
+    assert ops._stream(gpu) == ops._public_stream(gpu.index)
+    with torch.cuda.stream(side):
+        assert ops._stream(gpu) == ops._public_stream(gpu.index) == side.cuda_stream
+        monkeypatch.setattr(ops, "_raw_stream", ops._public_stream)       # as with a torch that lacks the short way
+        x = torch.randn(3, 64, device=gpu)
+        got = ops.rmsnorm(x, torch.ones(64, device=gpu), 1e-6)
+    torch.cuda.synchronize()
+    want = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6)
+    assert ((got - want).abs() <= 40 * 2.0 ** -24 * want.abs().amax()).all()  # 64 squares, a root, two products in fp32
